@@ -270,6 +270,40 @@ typedef struct {
 int llm_attn_decode_rope_batch_dev(const uint16_t *qkv_dev, int ldq, const llm_batch_desc *desc_dev, size_t cache_offset,
                                    int batch, int long_form, uint16_t *out_dev, int ldo, const float *table_dev, int n_heads,
                                    int n_kv_heads, int head_dim, int max_pos, void *workspace_dev, llm_stream_t stream);
+/* The step of `batch` (<= 16) sequences that share their first positions -- several answers to one prompt: cache rows of
+ * positions 0..prefix_len-1 are read once for the whole batch from one prefix cache ([n_kv_heads][prefix_max_pos][head_dim],
+ * V transposed like every V cache), the others from each sequence's own.  Otherwise llm_attn_decode_rope_batch: raw
+ * projection rows in, RoPE for position positions[z] >= prefix_len, K and V of the new token appended to the own cache,
+ * attention over positions 0..positions[z].
+ * Row r of every own cache ([n_kv_heads][max_pos][head_dim]) holds position row0 + r, 0 <= row0 <= prefix_len: 0 for caches
+ * that hold the prefix too (their rows below prefix_len are not read), prefix_len for caches that hold the answers only.
+ * positions[z] < row0 + max_pos; table_dev covers row0 + max_pos positions.  The prefix cache may be one of the own caches
+ * (with row0 = 0); own caches are distinct.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
+ * 2 GiB.  Rows that hold no position yet may hold anything, NaN included.
+ * Arithmetic: queries and the new key are rounded to fp16 after the rotation (llm_rope's results), products on the matrix
+ * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32.  The order of the sums depends on the
+ * lengths only: equal calls give equal bits.
+ * workspace: llm_attn_shared_workspace_bytes, zeroed once with llm_fill_zero before its first use (every call leaves it
+ * reusable, by calls of other shapes too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured graphs.
+ * No counterpart in the reference (it serves one sequence). */
+size_t llm_attn_shared_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int batch);
+int llm_attn_decode_rope_shared(const uint16_t *qkv_dev, int ldq, const uint16_t *k_prefix_dev, const uint16_t *v_prefix_dev,
+                                int prefix_len, int prefix_max_pos, uint16_t *const *k_caches, uint16_t *const *v_caches,
+                                const int *positions, int row0, int batch, uint16_t *out_dev, int ldo, const float *table_dev,
+                                int n_heads, int n_kv_heads, int head_dim, int max_pos, void *workspace_dev, llm_stream_t stream);
+/* The same with caches, lengths and positions read from an llm_shared_desc in device memory when the kernels run (for
+ * captured steps).  prefix_offset and cache_offset are added, in elements, to the prefix and own cache pointers.  The launch
+ * is sized for prefixes of up to max_prefix positions and sequences with up to max_tail rows behind it: a descriptor's
+ * longer prefix or tail, and positions outside the caches, are clamped to what is served. */
+typedef struct {
+    const uint16_t *k_prefix, *v_prefix;
+    int32_t prefix_len, row0;
+    llm_batch_desc seq; /* own caches and positions */
+} llm_shared_desc;
+int llm_attn_decode_rope_shared_dev(const uint16_t *qkv_dev, int ldq, const llm_shared_desc *desc_dev, size_t prefix_offset,
+                                    size_t cache_offset, int max_prefix, int prefix_max_pos, int max_tail, int batch,
+                                    uint16_t *out_dev, int ldo, const float *table_dev, int n_heads, int n_kv_heads,
+                                    int head_dim, int max_pos, void *workspace_dev, llm_stream_t stream);
 /* Same attention for T query rows at positions pos0..pos0+T-1 (prompt pass),
  * streaming softmax on MFMA tiles; never materialises [H,T,T].
  * q: [T, ldq] with head h at columns h*hd; out: [T, ldo].  Cache rows beyond
@@ -287,6 +321,39 @@ int llm_attn_prefill_rope_q_supported(int T, int n_heads, int n_kv_heads, int he
 int llm_attn_prefill_rope_q(const uint16_t *q_dev, int ldq, const uint16_t *k_cache_dev, const uint16_t *v_cache_dev,
                             uint16_t *out_dev, int ldo, int T, int pos0, const float *table_dev, int n_heads,
                             int n_kv_heads, int head_dim, int max_pos, llm_stream_t stream);
+
+/* ---- cache rows of other sequences ------------------------------------------------------------------ */
+/* Copies rows src_row..src_row+n_rows-1 of a K/V cache to rows dst_row.. of n_dst (1..16) other caches, all layers in one
+ * launch, every source row read once: a prompt's rows for each of its answers, an answer that branches, an answer that joins
+ * its prompt.  Layouts as the engine's: K [n_layers][n_kv_heads][max_pos][head_dim], V [n_layers][n_kv_heads][head_dim][max_pos],
+ * the same number of layers, heads and dims on both sides; src_max_pos and dst_max_pos (multiples of 64) may differ, and so
+ * may src_row and dst_row.  Bits are copied as they are: a row keeps the rotation of the position it was computed for, so a
+ * row number may only change where the position does not (a cache whose row 0 is not position 0).  Nothing else of the
+ * destinations is written.  A destination may be the source cache itself when the two ranges of rows are apart; any other
+ * memory in common is refused.  head_dim % 8 == 0, pointers 16-byte aligned; k_dsts/v_dsts are host arrays of device pointers.
+ * No counterpart in the reference. */
+int llm_kv_fork(const uint16_t *k_src_dev, const uint16_t *v_src_dev, int src_max_pos, int src_row, uint16_t *const *k_dsts,
+                uint16_t *const *v_dsts, int n_dst, int dst_max_pos, int dst_row, int n_rows, int n_layers, int n_kv_heads,
+                int head_dim, llm_stream_t stream);
+
+/* ---- log probabilities ---------------------------------------------------------------------------------- */
+/* For every row of fp16 logits ([rows, ld], vocab columns used; rows may start at any element): with y = logit / temperature,
+ *   logprob_dev[row][i] = y[ids[row][i]] - logsumexp(y)   for n_ids (0..16) given tokens, NaN for an id outside [0, vocab)
+ *   entropy_dev[row]    = -sum p ln p,  p = softmax(y)
+ *   top_ids_dev[row][j], top_logprob_dev[row][j]: the k (0..32, at most vocab) tokens of largest logit and their log
+ *   probabilities, largest first, the lowest id first among equal logits.
+ * A logit of -inf is a token of probability 0: log probability -inf, never an alternative (id -1, -inf fill the places that
+ * are left).  A row of -inf only: log probabilities -inf, entropy 0, no alternatives.  A row that holds a NaN or +inf has no
+ * distribution: NaN in every float, -1 in every id.  Statistics are fp32, in an order that depends on the sizes only.
+ * workspace: llm_logprobs_workspace_bytes, 16-byte aligned, zeroed once with llm_fill_zero before its first use (every call
+ * leaves it reusable, by calls of other shapes too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured graphs.
+ * No counterpart in the reference (its sampler keeps probabilities on the host, src/inference/inference.cu:1030-1061). */
+#define LLM_LOGPROBS_MAX_TOP 32
+#define LLM_LOGPROBS_MAX_IDS 16
+size_t llm_logprobs_workspace_bytes(int rows, int vocab, int k);
+int llm_logprobs(const uint16_t *logits_dev, int ld, int rows, int vocab, float temperature, const int32_t *ids_dev, int n_ids,
+                 float *logprob_dev, float *entropy_dev, int k, int32_t *top_ids_dev, float *top_logprob_dev,
+                 void *workspace_dev, llm_stream_t stream);
 
 /* ---- sampler candidates --------------------------------------------------------------------------- */
 /* Device half of sample_next_token (src/inference/inference.cu:1030-1161): what temperature_softmax's

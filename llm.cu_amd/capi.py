@@ -140,6 +140,12 @@ HIP_ABI = {
     "llm_attn_prefill": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "llm_attn_prefill_rope_q_supported": (_i, [_i, _i, _i, _i, _i]),
     "llm_attn_prefill_rope_q": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
+    "llm_attn_shared_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "llm_attn_decode_rope_shared": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "llm_attn_decode_rope_shared_dev": (_i, [_vp, _i, _vp, _sz, _sz, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "llm_kv_fork": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "llm_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
+    "llm_logprobs": (_i, [_vp, _i, _i, _i, C.c_float, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
     "llm_lmhead_workspace_bytes": (_sz, [_i]),
     "llm_lmhead_argmax": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "llm_argmax_f16": (_i, [_vp, _i, _vp, _vp, _vp]),

@@ -342,3 +342,93 @@ def attn_decode_rope_oproj(qkv, kc, vc, pos, n_heads, n_kv_heads, head_dim, w, r
         assert spin_limit >= 0 or res is None or all(np.array_equal(x, y) for x, y in zip(res, out)), "repeat %d differs" % r
         res = out
     return res + (int(tmo.download()[0]),)
+
+
+def _pointers(bufs):
+    return (C.c_void_p * len(bufs))(*[b.ptr for b in bufs])
+
+
+def _zeroed(nbytes):
+    buf = DevBuf(((nbytes + 3) // 4,), np.uint32)
+    buf.zero()
+    return buf
+
+
+class SharedDesc(C.Structure):
+    """llm_shared_desc"""
+    _fields_ = [("k_prefix", C.c_void_p), ("v_prefix", C.c_void_p), ("prefix_len", C.c_int32), ("row0", C.c_int32),
+                ("k_cache", C.c_void_p * 16), ("v_cache", C.c_void_p * 16), ("pos", C.c_int32 * 16)]
+
+
+def attn_decode_rope_shared(qkv, k_prefix, v_prefix, prefix_len, kcs, vcs, positions, row0, n_heads, n_kv_heads, head_dim,
+                            theta=500000.0, ldo=None, dev=False, max_prefix=None, max_tail=None, repeats=1):
+    """llm_attn_decode_rope_shared (dev: the _dev form, sized for max_prefix and max_tail or for what the descriptor holds).
+    qkv [B, ldq]; kcs [B, Hkv, max_pos, hd], vcs [B, Hkv, hd, max_pos]; k_prefix may be None (no prefix) or an int z: the own
+    cache of sequence z.  Returns (out [B, ldo], K caches, V caches)."""
+    qkv, kcs, vcs = _u16(qkv), _u16(kcs), _u16(vcs)
+    B, ldq = qkv.shape
+    max_pos = kcs.shape[2]
+    d_q = DevBuf.from_host(qkv)
+    d_ks, d_vs = [DevBuf.from_host(k) for k in kcs], [DevBuf.from_host(v) for v in vcs]
+    if k_prefix is None:
+        d_kp, d_vp, prefix_max = None, None, 0
+    elif isinstance(k_prefix, int):
+        d_kp, d_vp, prefix_max = d_ks[k_prefix], d_vs[k_prefix], max_pos
+    else:
+        d_kp, d_vp, prefix_max = DevBuf.from_host(_u16(k_prefix)), DevBuf.from_host(_u16(v_prefix)), k_prefix.shape[1]
+    d_t = DevBuf.from_host(rope_table(row0 + max_pos, head_dim, theta))
+    ldo = n_heads * head_dim if ldo is None else ldo
+    d_o = DevBuf.from_host(np.full((B, ldo), 0x7e00, np.uint16))
+    d_ws = _zeroed(lib().llm_attn_shared_workspace_bytes(n_heads, n_kv_heads, head_dim, B))
+    kp, vp = d_kp.ptr if d_kp else None, d_vp.ptr if d_vp else None
+    for _ in range(repeats):  # the workspace is reusable without clearing
+        if dev:
+            desc = SharedDesc(kp, vp, prefix_len, row0, (C.c_void_p * 16)(*[b.ptr for b in d_ks]),
+                              (C.c_void_p * 16)(*[b.ptr for b in d_vs]), (C.c_int32 * 16)(*[int(p) for p in positions]))
+            d_desc = DevBuf.from_host(np.frombuffer(bytes(desc), np.uint8))
+            most = max(int(p) - prefix_len for p in positions)
+            check(lib().llm_attn_decode_rope_shared_dev(
+                d_q.ptr, ldq, d_desc.ptr, 0, 0, prefix_len if max_prefix is None else max_prefix, prefix_max,
+                most if max_tail is None else max_tail, B, d_o.ptr, ldo, d_t.ptr, n_heads, n_kv_heads, head_dim, max_pos,
+                d_ws.ptr, None))
+        else:
+            check(lib().llm_attn_decode_rope_shared(
+                d_q.ptr, ldq, kp, vp, prefix_len, prefix_max, _pointers(d_ks), _pointers(d_vs),
+                (C.c_int * B)(*[int(p) for p in positions]), row0, B, d_o.ptr, ldo, d_t.ptr, n_heads, n_kv_heads, head_dim,
+                max_pos, d_ws.ptr, None))
+    return d_o.download(), np.stack([b.download() for b in d_ks]), np.stack([b.download() for b in d_vs])
+
+
+def kv_fork(k_src, v_src, src_row, k_dsts, v_dsts, dst_row, n_rows):
+    """llm_kv_fork.  k_src [L, Hkv, max_pos, hd], v_src [L, Hkv, hd, max_pos]; k_dsts, v_dsts: arrays of such caches, or None for
+    a copy inside the source cache.  Returns (K caches, V caches) afterwards."""
+    k_src, v_src = _u16(k_src), _u16(v_src)
+    L, Hkv, src_max, hd = k_src.shape
+    d_k, d_v = DevBuf.from_host(k_src), DevBuf.from_host(v_src)
+    d_ks = [d_k] if k_dsts is None else [DevBuf.from_host(_u16(k)) for k in k_dsts]
+    d_vs = [d_v] if v_dsts is None else [DevBuf.from_host(_u16(v)) for v in v_dsts]
+    dst_max = d_ks[0].shape[2]
+    check(lib().llm_kv_fork(d_k.ptr, d_v.ptr, src_max, src_row, _pointers(d_ks), _pointers(d_vs), len(d_ks), dst_max, dst_row,
+                            n_rows, L, Hkv, hd, None))
+    return np.stack([b.download() for b in d_ks]), np.stack([b.download() for b in d_vs])
+
+
+def logprobs(logits, vocab=None, ids=None, k=0, temperature=1.0, offset=0, ws=None, repeats=1):
+    """llm_logprobs on a [rows, ld] array whose first `vocab` columns count, uploaded `offset` elements behind a 16-byte
+    boundary.  ids: [rows, n] or None.  Returns (logprob [rows, n], entropy [rows], top_ids [rows, k], top_logprob [rows, k])."""
+    logits = _u16(logits)
+    rows, ld = logits.shape
+    vocab = ld if vocab is None else vocab
+    ids = np.zeros((rows, 0), np.int32) if ids is None else np.ascontiguousarray(ids, dtype=np.int32).reshape(rows, -1)
+    n = ids.shape[1]
+    d_x = DevBuf.from_host(np.concatenate([np.full(offset, 0x7c00, np.uint16), logits.reshape(-1)]))
+    d_i = DevBuf.from_host(ids)
+    d_lp, d_h = DevBuf((rows, n), np.float32), DevBuf((rows,), np.float32)
+    d_ti, d_tl = DevBuf((rows, k), np.int32), DevBuf((rows, k), np.float32)
+    if ws is None:
+        ws = _zeroed(lib().llm_logprobs_workspace_bytes(rows, vocab, k))
+    for _ in range(repeats):
+        check(lib().llm_logprobs(d_x.ptr + 2 * offset, ld, rows, vocab, temperature, d_i.ptr if n else None, n,
+                                 d_lp.ptr if n else None, d_h.ptr, k, d_ti.ptr if k else None, d_tl.ptr if k else None, ws.ptr,
+                                 None))
+    return d_lp.download(), d_h.download(), d_ti.download(), d_tl.download()
