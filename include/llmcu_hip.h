@@ -326,7 +326,7 @@ int llm_attn_prefill_rope_q(const uint16_t *q_dev, int ldq, const uint16_t *k_ca
 /* Copies rows src_row..src_row+n_rows-1 of a K/V cache to rows dst_row.. of n_dst (1..16) other caches, all layers in one
  * launch, every source row read once: a prompt's rows for each of its answers, an answer that branches, an answer that joins
  * its prompt.  Layouts as the engine's: K [n_layers][n_kv_heads][max_pos][head_dim], V [n_layers][n_kv_heads][head_dim][max_pos],
- * the same number of layers, heads and dims on both sides; src_max_pos and dst_max_pos (multiples of 64) may differ, and so
+ * the same number of layers, heads and dims on both sides; src_max_pos and dst_max_pos (multiples of 64, at most 2^30) may differ, and so
  * may src_row and dst_row.  Bits are copied as they are: a row keeps the rotation of the position it was computed for, so a
  * row number may only change where the position does not (a cache whose row 0 is not position 0).  Nothing else of the
  * destinations is written.  A destination may be the source cache itself when the two ranges of rows are apart; any other

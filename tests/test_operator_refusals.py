@@ -83,7 +83,7 @@ SIZE = 2 * 32 * 8 * 128 * 256  # bytes of one half of a cache above
     (dict(ks=(None, A + 3 * BIG)), "destination 0"), (dict(vs=(A + 4 * BIG, None)), "destination 1"),
     (dict(n_dst=0), "destinations"), (dict(n_dst=17), "destinations"), (dict(n_dst=-1), "destinations"),
     (dict(L=0), "layers"), (dict(hkv=0), "layers"), (dict(L=65536, hkv=1), "layers"), (dict(hd=0), "head_dim"), (dict(hd=12), "head_dim"),
-    (dict(hd=1032), "head_dim"), (dict(smax=0), "multiples"), (dict(smax=65), "multiples"), (dict(dmax=100), "multiples"), (dict(dmax=-64), "multiples"),
+    (dict(hd=1032), "head_dim"), (dict(smax=0), "multiples"), (dict(smax=65), "multiples"), (dict(dmax=100), "multiples"), (dict(smax=(1 << 30) + 64), "2^30"), (dict(dmax=(1 << 30) + 64), "2^30"), (dict(dmax=-64), "multiples"),
     (dict(n=-1), "rows"), (dict(srow=-1), "rows"), (dict(srow=257), "rows"), (dict(srow=1, n=256), "rows"), (dict(srow=2 ** 31 - 1, n=2), "rows"),
     (dict(drow=-1), "rows"), (dict(drow=257), "rows"), (dict(drow=255, n=2), "rows"), (dict(drow=2 ** 31 - 1, n=2), "rows"),
     (dict(k=A + 2), "aligned"), (dict(v=A + 8), "aligned"), (dict(ks=(A + 2, A + 3 * BIG)), "destination 0"),
