@@ -113,7 +113,7 @@ def logprobs(pkg, **over):
 
 @pytest.mark.parametrize("over,text", [
     (dict(x=None), "null"), (dict(ids=None), "null"), (dict(lp=None), "null"), (dict(ent=None), "null"), (dict(ti=None), "null"), (dict(tl=None), "null"),
-    (dict(ws=None), "null"), (dict(rows=-1), "rows"), (dict(vocab=0), "rows"), (dict(ld=999), "ld"), (dict(t=0.0), "temperature"),
+    (dict(ws=None), "null"), (dict(rows=-1), "rows"), (dict(vocab=0), "rows"), (dict(vocab=(1 << 20) + 1, ld=1 << 21), "at most"), (dict(ld=999), "ld"), (dict(t=0.0), "temperature"),
     (dict(t=-1.0), "temperature"), (dict(t=float("nan")), "temperature"), (dict(t=float("inf")), "temperature"), (dict(t=1e-45), "temperature"),
     (dict(n=-1), "given"), (dict(n=17), "given"), (dict(k=-1), "top"), (dict(k=33), "top"), (dict(k=4, vocab=3), "top"), (dict(ws=A + 8), "aligned"),
     (dict(x=A + 1), "aligned"), (dict(ids=A + 2), "aligned"), (dict(ent=A + 1), "aligned"),
