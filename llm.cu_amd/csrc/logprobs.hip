@@ -3,15 +3,19 @@
 //   y = x / temperature, m = max y, S = sum exp(y - m)
 //   logprob(i) = (y_i - m) - ln S,   entropy = ln S - sum (y - m) exp(y - m) / S
 //
-// One pass over the logits: a row is cut into chunks, one workgroup holds a chunk in registers, takes the sums relative to each
-// wavefront's own maximum (no barrier between the loads and the exponentials) and picks the chunk's k best; the workgroup of a
-// row that finishes last joins the chunks.  Exponentials are base 2: 2^((x - m) c) with c = log2(e) / temperature, x - m exact
-// in fp32 for fp16 values of similar size, so nothing is lost at large logits or low temperatures.
+// One pass over the logits.  A row is cut into chunks, one workgroup each; its wavefronts go through the chunk's segments on
+// their own, the next segment's loads in flight while one is worked on, and meet at the end of the chunk only; the workgroup of
+// a row that finishes last joins the chunks.
 //
-// The k best (k <= 32) of a chunk without a sort: the k-th largest of the 64 lane maxima of a wavefront is a lower bound of the
-// chunk's k-th largest logit, found by bisection on 16-bit order keys (ballot and bit count, 16 steps); the few logits from
-// there up (about 1.2 k in random data) are listed in LDS and ranked by counting.  A listed logit is one 32-bit word, order key
-// above the complement of its place, so that a larger word is a larger logit or an equal one further in front.
+// Sums: exponentials are base 2, 2^(x c - R) with c = log2(e) / temperature and R = fl(m c) for the largest logit m so far: one
+// fused operation on the fp16 value, exact before its rounding.  A larger m rescales the lane's sums.  Parts are joined by their
+// R; what the rounding of m c shifted goes out again at the end.
+//
+// The k best (k <= 32) without a sort: the k-th largest of a wavefront's 64 running lane maxima is a lower bound of its k-th
+// largest logit, found by bisection on 16-bit order keys (ballot and bit count, 16 steps).  The few logits from there up are
+// appended to the wavefront's list in LDS; a list that would overflow (many equal logits, rising rows) is cut down to its k
+// best, after which only larger logits can enter, since equal ones further back lose.  A listed logit is a 64-bit word, order
+// key above the complement of its index.
 #include <cfloat>
 #include <cmath>
 
@@ -22,28 +26,35 @@
 #define LP_MAX_TOP LLM_LOGPROBS_MAX_TOP
 #define LP_MAX_IDS LLM_LOGPROBS_MAX_IDS
 #define LP_MAX_CHUNKS 64       // of a row: one lane each when they are joined
-#define LP_MAX_LOADS 8         // 16-byte loads per thread and chunk: 16384 logits
-#define LP_MAX_VOCAB (LP_MAX_CHUNKS * LP_THREADS * 8 * LP_MAX_LOADS)
+#define LP_MAX_VOCAB (1 << 20)
 #define LP_SLICE 4096          // rows per launch: a counter each at the front of the workspace
-#define LP_MERGE (LP_MAX_CHUNKS * LP_MAX_TOP / LP_THREADS) // listed logits per thread when chunks are joined
+#define LP_LIST 576            // words of a wavefront's list: a row of 16-byte loads (512 logits), and the k best
+#define LP_JOIN (LP_MAX_CHUNKS * LP_MAX_TOP / LP_THREADS) // listed logits per thread when chunks are joined
 #define LP_LOWEST 0x0400u      // order key of -65504, the lowest logit that has a probability
+
+typedef unsigned long long lp_word;
 
 struct LpArgs {
     const half_t *x;
     size_t ld;
-    int vocab, n_ids, k, chunks;
+    int vocab, n_ids, k, chunks, chunk_len;
     float inv_t;
     const int32_t *ids;
     float *logprob, *entropy, *top;
     int32_t *top_ids;
     int *counters;
-    uint32_t *stats;    // [row][chunk][4]: m, S, sum y 2^y (relative to m, base 2) as bits
-    uint32_t *listed;   // [row][chunk][k]
+    lp_word *listed;    // [row][chunk][k]
+    uint32_t *stats;    // [row][chunk][4]: m, S, sum y 2^y as bits
 };
 
 struct LpStats {
-    float m, s, t;
+    float m, s, t; // largest logit, sum of 2^y, sum of y 2^y with y = x c - fl(m c)
 };
+
+__device__ __forceinline__ void lp_put(uint32_t *p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint32_t lp_get(const uint32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void lp_put(lp_word *p, lp_word v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ lp_word lp_get(const lp_word *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // eight logits from any element of a row
 __device__ __forceinline__ half8_t lp_load8(const half_t *p) {
@@ -56,15 +67,15 @@ __device__ __forceinline__ uint32_t lp_key(half_t h) { return f16_order_key(__bu
 __device__ __forceinline__ half_t lp_value(uint32_t key) { // the logit of an order key (+0 for either zero)
     return __builtin_bit_cast(half_t, (uint16_t)(key >= 0x8000u ? key - 0x8000u : 0xffffu - key));
 }
+__device__ __forceinline__ lp_word lp_make(half_t h, int index) { return (lp_word)lp_key(h) << 32 | (uint32_t)~index; }
+__device__ __forceinline__ uint32_t lp_word_key(lp_word w) { return (uint32_t)(w >> 32); }
 
-__device__ __forceinline__ void lp_put(uint32_t *p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint32_t lp_get(const uint32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float lp_ref(float m, float c) { return m == -INFINITY ? 0.f : m * c; }
 
-// a part's sums relative to a larger maximum M
+// sums relative to the reference of a larger maximum M
 __device__ __forceinline__ LpStats lp_rebase(LpStats p, float M, float c) {
-    if (p.s == 0.f) return {M, 0.f, 0.f}; // nothing in this part (its maximum is -inf)
-    const float d = (p.m - M) * c, f = __builtin_amdgcn_exp2f(d);
-    return {M, f * p.s, f == 0.f ? 0.f : f * (p.t + d * p.s)}; // d may be -inf at the lowest temperatures
+    const float d = lp_ref(p.m, c) - lp_ref(M, c), f = p.s == 0.f ? 0.f : __builtin_amdgcn_exp2f(d);
+    return {M, f * p.s, f == 0.f ? 0.f : f * (p.t + d * p.s)};
 }
 
 // k-th largest of the lanes' keys (0: fewer than k lanes have one)
@@ -78,108 +89,165 @@ __device__ __forceinline__ uint32_t lp_kth_key(uint32_t key, int k) {
     return t;
 }
 
-__device__ __forceinline__ uint32_t lp_wave_max(uint32_t v) {
-    for (int o = 32; o; o >>= 1) {
-        const uint32_t q = (uint32_t)__shfl_xor((int)v, o);
-        v = q > v ? q : v;
-    }
-    return v;
+// LDS written by some lanes of a wavefront, read by others: its operations are carried out in order, the compiler keeps theirs
+__device__ __forceinline__ void lp_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// The k largest of the n distinct words in list, largest first, into best (zeros behind the last one).  All threads call it;
-// best is ready behind the barrier it ends with.
-__device__ __forceinline__ void lp_rank(const uint32_t *list, int n, int k, uint32_t *best, uint32_t *red) {
+// Appends the lanes' words (0: none) to the wavefront's list of n words; returns the new length.
+__device__ __forceinline__ int lp_append(lp_word *list, int n, lp_word w) {
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(w != 0ull);
+    const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+    if (w) list[n + before] = w;
+    return n + __popcll(who);
+}
+
+// The k largest of a wavefront's n <= LP_LIST distinct words to the front of its list, largest first, zeros behind the last.
+__device__ __forceinline__ void lp_cut(lp_word *list, int n, int k) {
+    const int lane = threadIdx.x % 64;
+    lp_wave_sync();
+    if (n <= 128) {
+        const lp_word a = lane < n ? list[lane] : 0ull, b = lane + 64 < n ? list[lane + 64] : 0ull;
+        int ra = 0, rb = 0;
+        for (int j = 0; j < n; ++j) {
+            const lp_word w = list[j];
+            ra += w > a;
+            rb += w > b;
+        }
+        lp_wave_sync();
+        if (a && ra < k) list[ra] = a;
+        if (b && rb < k) list[rb] = b;
+    } else { // their maximum, k times
+        lp_word w[LP_LIST / 64];
+#pragma unroll
+        for (int i = 0; i < LP_LIST / 64; ++i) w[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0ull;
+        lp_wave_sync();
+        for (int r = 0; r < k; ++r) {
+            lp_word top = 0ull;
+#pragma unroll
+            for (int i = 0; i < LP_LIST / 64; ++i) top = w[i] > top ? w[i] : top;
+            for (int o = 32; o; o >>= 1) {
+                const lp_word q = __shfl_xor(top, o);
+                top = q > top ? q : top;
+            }
+#pragma unroll
+            for (int i = 0; i < LP_LIST / 64; ++i) w[i] = w[i] == top ? 0ull : w[i];
+            if (lane == 0) list[r] = top;
+        }
+    }
+    if (lane >= n && lane < k) list[lane] = 0ull;
+    lp_wave_sync();
+}
+
+// The wavefronts' lists (k words each, cut) into best, largest first.  All threads call it, behind a barrier.
+__device__ __forceinline__ void lp_join_waves(const lp_word *lists, int k, lp_word *best) {
     const int tid = threadIdx.x;
-    if (tid < k) best[tid] = 0u;
+    if (tid < k) best[tid] = 0ull;
     __syncthreads();
-    if (n <= 2 * LP_THREADS) {
-        for (int i = tid; i < n; i += LP_THREADS) {
-            const uint32_t v = list[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > v;
-            if (rank < k) best[rank] = v;
-        }
-        __syncthreads();
-        return;
+    if (tid < LP_WAVES * k) {
+        const lp_word mine = lists[tid / k * LP_LIST + tid % k];
+        int rank = 0;
+        for (int w = 0; w < LP_WAVES; ++w)
+            for (int j = 0; j < k; ++j) rank += lists[w * LP_LIST + j] > mine;
+        if (mine && rank < k) best[rank] = mine;
     }
-    uint32_t below = 0xffffffffu; // many words: their maximum, k times
-    for (int r = 0; r < k; ++r) {
-        uint32_t v = 0;
-        for (int i = tid; i < n; i += LP_THREADS) {
-            const uint32_t w = list[i];
-            v = w < below && w > v ? w : v;
-        }
-        v = lp_wave_max(v);
-        if (tid % 64 == 0) red[tid / 64] = v;
-        __syncthreads();
-        for (int w = 0; w < LP_WAVES; ++w) v = red[w] > v ? red[w] : v;
-        if (tid == 0) best[r] = v;
-        below = v;
-        __syncthreads();
-        if (v == 0) break;
-    }
+    __syncthreads();
 }
 
+// NL 16-byte loads per lane and segment.
 template <int NL>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
-    constexpr int CHUNK = LP_THREADS * 8 * NL;
-    // A lane whose maximum is below the bound lists nothing, and fewer than k lanes of a wavefront have a maximum above it: more
-    // than this many logits above the bound cannot be.
-    constexpr int LIST = (LP_MAX_TOP * 8 * NL * LP_WAVES > LP_MAX_CHUNKS * LP_MAX_TOP) ? LP_MAX_TOP * 8 * NL * LP_WAVES : LP_MAX_CHUNKS * LP_MAX_TOP;
-    __shared__ uint32_t list[LIST], best[LP_MAX_TOP], red[LP_WAVES], listed_n;
+    constexpr int SEG = 64 * 8 * NL;
+    extern __shared__ lp_word lists[]; // LP_WAVES lists of LP_LIST words when k > 0
+    __shared__ lp_word best[LP_MAX_TOP];
     __shared__ float part[LP_WAVES][3];
     __shared__ int is_last;
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunk = blockIdx.x, k = a.k;
     const size_t row = blockIdx.y;
     const half_t *x = a.x + row * a.ld;
     const float c = a.inv_t * 1.44269504088896341f;
-
-    // ---- 1. the chunk into registers, -inf behind the end of the row --------------------------------------------------
     const half_t ninf = __builtin_bit_cast(half_t, (uint16_t)0xfc00u);
-    half8_t v[NL];
+    lp_word *list = lists + wave * LP_LIST;
+
+    // ---- 1. the wavefront's segments: wave, wave + LP_WAVES, ... of the chunk ---------------------------------------------
+    const int begin = chunk * a.chunk_len, end = begin + a.chunk_len < a.vocab ? begin + a.chunk_len : a.vocab;
+    LpStats st = {-INFINITY, 0.f, 0.f}; // m of the wavefront, sums of the lane
+    half_t lane_best = ninf;
+    uint32_t bound = LP_LOWEST; // order key from which on a logit is listed
+    int n = 0;
+    half8_t v[NL], next[NL];
+    auto load = [&](half8_t (&d)[NL], int s0) __attribute__((always_inline)) { // -inf behind the end
 #pragma unroll
-    for (int u = 0; u < NL; ++u) {
-        const int i = chunk * CHUNK + (u * LP_THREADS + tid) * 8;
-        if (i + 8 <= a.vocab) {
-            v[u] = lp_load8(x + i);
-        } else {
+        for (int u = 0; u < NL; ++u) {
+            const int i = s0 + (u * 64 + lane) * 8;
+            if (i + 8 <= end) {
+                d[u] = lp_load8(x + i);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = i + e < a.vocab ? x[i + e] : ninf;
+                for (int e = 0; e < 8; ++e) d[u][e] = i + e < end ? x[i + e] : ninf;
+            }
         }
-    }
-    // ---- 2. the lane's and the wavefront's maximum, the sums relative to the latter -----------------------------------
-    half8_t m8 = v[0];
+    };
+    int s0 = begin + wave * SEG;
+    if (s0 < end) load(v, s0);
+    for (; s0 < end; s0 += LP_WAVES * SEG) {
+        const bool more = s0 + LP_WAVES * SEG < end;
+        if (more) load(next, s0 + LP_WAVES * SEG);
+        half8_t m8 = v[0];
 #pragma unroll
-    for (int u = 1; u < NL; ++u) m8 = __builtin_elementwise_max(m8, v[u]);
-    half_t lane_max = ninf; // a NaN loses against any number here; the sums find it
+        for (int u = 1; u < NL; ++u) m8 = __builtin_elementwise_max(m8, v[u]);
+        half_t top = ninf; // a NaN loses against any number here; the sums find it
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lane_max = m8[e] > lane_max ? m8[e] : lane_max;
-    LpStats st = {wave_max((float)lane_max), 0.f, 0.f};
-    {
-        const float m0 = st.m == -INFINITY ? 0.f : st.m;
+        for (int e = 0; e < 8; ++e) top = m8[e] > top ? m8[e] : top;
+        if (__builtin_amdgcn_ballot_w64((float)top > st.m)) st = lp_rebase(st, fmaxf(st.m, wave_max((float)top)), c);
+        const float ref = lp_ref(st.m, c);
 #pragma unroll
         for (int u = 0; u < NL; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = ((float)v[u][e] - m0) * c, p = __builtin_amdgcn_exp2f(y);
+                const float y = fmaf((float)v[u][e], c, -ref), p = __builtin_amdgcn_exp2f(y);
                 st.s += p;
                 st.t = fmaf(fmaxf(y, -FLT_MAX), p, st.t); // -inf times zero is zero here; a NaN is in p already
             }
-        st.s = wave_sum(st.s);
-        st.t = wave_sum(st.t);
+        if (k > 0 && __builtin_amdgcn_ballot_w64(top >= lp_value(bound))) {
+            lane_best = top > lane_best ? top : lane_best;
+            const uint32_t kth = lp_kth_key(lane_best == ninf ? 0u : lp_key(lane_best), k);
+            bound = kth > bound ? kth : bound;
+            half_t from = lp_value(bound);
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                int count = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) count += __popcll(__builtin_amdgcn_ballot_w64(v[u][e] >= from));
+                if (count == 0) continue;
+                if (n + count > LP_LIST) {
+                    lp_cut(list, n, k);
+                    n = n < k ? n : k;
+                    if (n == k) { // an equal logit further back is not among the k best
+                        const uint32_t above = lp_word_key(list[k - 1]) + 1u;
+                        bound = above > bound ? above : bound;
+                        from = lp_value(bound);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    n = lp_append(list, n, v[u][e] >= from ? lp_make(v[u][e], s0 + (u * 64 + lane) * 8 + e) : 0ull);
+            }
+        }
+        if (more)
+#pragma unroll
+            for (int u = 0; u < NL; ++u) v[u] = next[u];
     }
+    // ---- 2. the workgroup's wavefronts -------------------------------------------------------------------------------------
+    st.s = wave_sum(st.s);
+    st.t = wave_sum(st.t);
     if (lane == 0) {
         part[wave][0] = st.m;
         part[wave][1] = st.s;
         part[wave][2] = st.t;
     }
-    // ---- 3. the k best of the chunk ------------------------------------------------------------------------------------
-    if (k > 0) {
-        uint32_t bound = lane_max == ninf ? 0u : lp_key(lane_max);
-        bound = k == 1 ? lp_wave_max(bound) : lp_kth_key(bound, k);
-        if (lane == 0) red[wave] = bound;
-        if (tid == 0) listed_n = 0u;
-    }
+    if (k > 0) lp_cut(list, n, k);
     __syncthreads();
     float M = part[0][0];
 #pragma unroll
@@ -191,72 +259,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         st.s += p.s;
         st.t += p.t;
     }
-    if (k > 0) {
-        uint32_t bound = LP_LOWEST; // no logit of probability zero
-#pragma unroll
-        for (int w = 0; w < LP_WAVES; ++w) bound = red[w] > bound ? red[w] : bound;
-        const half_t bv = lp_value(bound);
-        auto word = [&](int u, int e) { return lp_key(v[u][e]) << 16 | (uint32_t)(0xffff - ((u * LP_THREADS + tid) * 8 + e)); };
-        if (lane_max >= bv) {
-#pragma unroll
-            for (int u = 0; u < NL; ++u)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (v[u][e] >= bv) {
-                        const uint32_t at = atomicAdd(&listed_n, 1u);
-                        if (at < LIST) list[at] = word(u, e);
-                    }
-        }
-        __syncthreads();
-        int n = (int)listed_n;
-        if (n > LIST) { // many logits equal to the bound: only those above it, then as many equal ones as are missing, in order
-            __syncthreads();
-            if (tid == 0) listed_n = 0u;
-            __syncthreads();
-            if (lane_max > bv) {
-#pragma unroll
-                for (int u = 0; u < NL; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (v[u][e] > bv) list[atomicAdd(&listed_n, 1u)] = word(u, e);
-            }
-            __syncthreads();
-            n = (int)listed_n;
-            const int above = n;
-            for (int u = 0; u < NL && n < k; ++u) { // n is the same in every thread
-                int mine = 0;
-                half8_t vu = v[0];
-#pragma unroll
-                for (int w = 1; w < NL; ++w) vu = w == u ? v[w] : vu;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mine += vu[e] == bv;
-                int before = mine; // inclusive over the wavefront's lanes
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int q = __shfl_up(before, o);
-                    if (lane >= o) before += q;
-                }
-                if (lane == 63) red[wave] = (uint32_t)before;
-                __syncthreads();
-                int at = n + before - mine, total = 0;
-                for (int w = 0; w < LP_WAVES; ++w) {
-                    if (w < wave) at += (int)red[w];
-                    total += (int)red[w];
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (vu[e] == bv) {
-                        if (at < k) list[at] = bound << 16 | (uint32_t)(0xffff - ((u * LP_THREADS + tid) * 8 + e));
-                        ++at;
-                    }
-                n += total;
-                __syncthreads();
-            }
-            if (above < k && n > k) n = k;
-        }
-        lp_rank(list, n, k, best, red);
-    }
-    // ---- 4. several chunks: leave this one's result; the row's last workgroup goes on -------------------------------------
+    if (k > 0) lp_join_waves(lists, k, best);
+    // ---- 3. several chunks: leave this one's result; the row's last workgroup goes on -------------------------------------
     if (a.chunks > 1) {
         // Handed over by device-scope stores (written through to where every XCD reads them) that are complete before the
         // counter moves, and device-scope loads: a fence in each of thousands of workgroups would write the L2 back each time
@@ -277,42 +281,31 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         M = wave_max(mine[0]);
         const LpStats p = lp_rebase({mine[0], mine[1], mine[2]}, M, c);
         st = {M, wave_sum(p.s), wave_sum(p.t)};
-        if (k > 0) {
-            // the chunks' lists as one, in the order of the row; the same bound as above
-            const uint32_t *listed = a.listed + row * a.chunks * k;
+        if (k > 0) { // the chunks' lists, with a bound as above
+            const lp_word *listed = a.listed + row * a.chunks * k;
             const int total = a.chunks * k;
-            uint32_t w[LP_MERGE], lane_best = 0u;
+            lp_word w[LP_JOIN], top = 0ull;
 #pragma unroll
-            for (int j = 0; j < LP_MERGE; ++j) {
+            for (int j = 0; j < LP_JOIN; ++j) {
                 const int q = tid + LP_THREADS * j;
-                const uint32_t e = q < total ? lp_get(listed + q) : 0u;
-                w[j] = e ? (e & 0xffff0000u) | (uint32_t)(0xffff - q) : 0u;
-                lane_best = w[j] > lane_best ? w[j] : lane_best;
+                w[j] = q < total ? lp_get(listed + q) : 0ull;
+                top = w[j] > top ? w[j] : top;
             }
-            const uint32_t bound_w = lp_kth_key(lane_best >> 16, k);
-            if (lane == 0) red[wave] = bound_w;
-            if (tid == 0) listed_n = 0u;
-            __syncthreads();
-            uint32_t bound = LP_LOWEST;
+            const uint32_t kth = lp_kth_key(lp_word_key(top), k);
+            n = 0;
 #pragma unroll
-            for (int i = 0; i < LP_WAVES; ++i) bound = red[i] > bound ? red[i] : bound;
-#pragma unroll
-            for (int j = 0; j < LP_MERGE; ++j)
-                if (w[j] >> 16 >= bound) list[atomicAdd(&listed_n, 1u)] = w[j];
+            for (int j = 0; j < LP_JOIN; ++j) n = lp_append(list, n, lp_word_key(w[j]) >= kth ? w[j] : 0ull);
+            lp_cut(list, n, k);
             __syncthreads();
-            lp_rank(list, (int)listed_n, k, best, red);
-            if (tid < k && best[tid]) { // back to the place in the row
-                const int q = 0xffff - (int)(best[tid] & 0xffffu);
-                list[tid] = (uint32_t)(q / k * CHUNK) + 0xffffu - (lp_get(listed + q) & 0xffffu);
-            }
+            lp_join_waves(lists, k, best);
         }
-    } else if (tid < k) {
-        list[tid] = 0xffffu - (best[tid] & 0xffffu);
     }
-    // ---- 5. results ------------------------------------------------------------------------------------------------------
+    // ---- 4. results ------------------------------------------------------------------------------------------------------
     const bool invalid = st.s != st.s, none = st.s == 0.f;
-    const float m0 = none ? 0.f : st.m, log_s = none ? 0.f : logf(st.s);
-    if (tid == 0) a.entropy[row] = invalid ? NAN : none ? 0.f : log_s - st.t / st.s * 0.693147180559945309f;
+    const float m0 = none ? 0.f : st.m, off = fmaf(m0, c, -lp_ref(m0, c)); // sums stand at 2^off times their value for m c itself
+    const float mean = none ? 0.f : (st.t / st.s - off) * 0.693147180559945309f;
+    const float log_s = none ? 0.f : logf(st.s) - off * 0.693147180559945309f;
+    if (tid == 0) a.entropy[row] = invalid ? NAN : log_s - mean;
     if (tid < a.n_ids) {
         const int id = a.ids[row * a.n_ids + tid];
         float lp = NAN;
@@ -320,30 +313,33 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         a.logprob[row * a.n_ids + tid] = lp;
     }
     if (tid < k) {
-        const bool some = best[tid] != 0u && !invalid;
-        a.top_ids[row * k + tid] = some ? (int)list[tid] : -1;
-        a.top[row * k + tid] = invalid ? NAN : some ? ((float)lp_value(best[tid] >> 16) - m0) * a.inv_t - log_s : -INFINITY;
+        const bool some = best[tid] != 0ull && !invalid;
+        a.top_ids[row * k + tid] = some ? (int)~(uint32_t)best[tid] : -1;
+        a.top[row * k + tid] = invalid ? NAN : some ? ((float)lp_value(lp_word_key(best[tid])) - m0) * a.inv_t - log_s : -INFINITY;
     }
 }
 
-// Loads per thread of a chunk.  Few rows are cut finely, so that their logits come from many compute units at once (at most
-// LP_MAX_CHUNKS pieces); many rows coarsely, so that less is joined.
-static int lp_loads(int rows, int vocab) {
-    int nl = 1;
-    while (nl < LP_MAX_LOADS) {
-        const int one = LP_THREADS * 8 * nl, chunks = (vocab + one - 1) / one, coarser = (vocab + 2 * one - 1) / (2 * one);
-        if (chunks <= LP_MAX_CHUNKS && (chunks == 1 || (long long)rows * coarser < 512)) break;
-        nl *= 2;
-    }
-    return nl;
-}
-static int lp_chunks(int rows, int vocab) {
-    const int one = LP_THREADS * 8 * lp_loads(rows, vocab);
-    return (vocab + one - 1) / one;
+// How a row is cut.  Few rows: finely, so that their logits come from many compute units at once, but into LP_MAX_CHUNKS pieces
+// at most; many rows: coarsely, so that less is joined.
+struct LpCut {
+    int nl, chunk_len, chunks;
+};
+static LpCut lp_cut_row(int rows, int vocab) {
+    const int target = 2048; // workgroups
+    int want = (target + rows - 1) / rows;
+    if (want > LP_MAX_CHUNKS) want = LP_MAX_CHUNKS;
+    int len = (vocab + want - 1) / want;
+    LpCut r = {};
+    r.nl = len <= 2048 ? 1 : len <= 4096 ? 2 : 4;
+    const int unit = LP_THREADS * 8 * r.nl;
+    r.chunk_len = (len + unit - 1) / unit * unit;
+    r.chunks = (vocab + r.chunk_len - 1) / r.chunk_len;
+    return r;
 }
 
 template <int NL> static void lp_launch(const LpArgs &a, int rows, hipStream_t s) {
-    logprobs_kernel<NL><<<dim3(a.chunks, rows), dim3(LP_THREADS), 0, s>>>(a);
+    const size_t smem = a.k > 0 ? sizeof(lp_word) * LP_WAVES * LP_LIST : 0;
+    logprobs_kernel<NL><<<dim3(a.chunks, rows), dim3(LP_THREADS), smem, s>>>(a);
 }
 
 extern "C" {
@@ -351,15 +347,15 @@ extern "C" {
 // counters of LP_SLICE rows, then the statistics and lists of one launch
 size_t llm_logprobs_workspace_bytes(int rows, int vocab, int k) {
     if (rows < 1 || vocab < 1 || vocab > LP_MAX_VOCAB || k < 0) return sizeof(int) * LP_SLICE;
-    const size_t n = (size_t)(rows < LP_SLICE ? rows : LP_SLICE) * lp_chunks(rows, vocab);
-    return sizeof(int) * LP_SLICE + n * sizeof(uint32_t) * (4 + k);
+    const size_t n = (size_t)(rows < LP_SLICE ? rows : LP_SLICE) * lp_cut_row(rows, vocab).chunks;
+    return sizeof(int) * LP_SLICE + n * (sizeof(uint32_t) * 4 + sizeof(lp_word) * k);
 }
 
 int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temperature, const int32_t *ids, int n_ids,
                  float *logprob, float *entropy, int k, int32_t *top_ids, float *top_logprob, void *workspace, llm_stream_t stream) {
     LLM_REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab, "llm_logprobs: %d rows of %d logits, ld=%d", rows, vocab, ld);
     LLM_REQUIRE(vocab <= LP_MAX_VOCAB, "llm_logprobs: %d logits per row (at most %d)", vocab, LP_MAX_VOCAB);
-    LLM_REQUIRE(temperature >= FLT_MIN && temperature <= FLT_MAX, "llm_logprobs: temperature %g", (double)temperature);
+    LLM_REQUIRE(temperature >= 1e-30f && temperature <= FLT_MAX, "llm_logprobs: temperature %g (at least 1e-30)", (double)temperature);
     LLM_REQUIRE(n_ids >= 0 && n_ids <= LP_MAX_IDS, "llm_logprobs: %d given tokens per row (0..%d)", n_ids, LP_MAX_IDS);
     LLM_REQUIRE(k >= 0 && k <= LP_MAX_TOP && k <= vocab, "llm_logprobs: top %d of %d (at most %d)", k, vocab, LP_MAX_TOP);
     LLM_REQUIRE(logits && entropy && workspace && (n_ids == 0 || (ids && logprob)) && (k == 0 || (top_ids && top_logprob)),
@@ -372,26 +368,25 @@ int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temp
     a.vocab = vocab;
     a.n_ids = n_ids;
     a.k = k;
-    a.chunks = lp_chunks(rows, vocab);
+    const LpCut cut = lp_cut_row(rows, vocab);
+    a.chunks = cut.chunks;
+    a.chunk_len = cut.chunk_len;
     a.inv_t = 1.f / temperature;
     a.counters = (int *)workspace;
     a.stats = (uint32_t *)workspace + LP_SLICE;
     hipStream_t s = (hipStream_t)stream;
     for (int r0 = 0; r0 < rows; r0 += LP_SLICE) {
         const int n = rows - r0 < LP_SLICE ? rows - r0 : LP_SLICE;
-        a.listed = a.stats + (size_t)n * a.chunks * 4;
+        a.listed = (lp_word *)(a.stats + (size_t)n * a.chunks * 4);
         a.x = (const half_t *)logits + (size_t)r0 * ld;
         a.ids = ids + (size_t)r0 * n_ids;
         a.logprob = logprob + (size_t)r0 * n_ids;
         a.entropy = entropy + r0;
         a.top_ids = top_ids + (size_t)r0 * k;
         a.top = top_logprob + (size_t)r0 * k;
-        switch (lp_loads(rows, vocab)) {
-        case 1: lp_launch<1>(a, n, s); break;
-        case 2: lp_launch<2>(a, n, s); break;
-        case 4: lp_launch<4>(a, n, s); break;
-        default: lp_launch<8>(a, n, s); break;
-        }
+        if (cut.nl == 1) lp_launch<1>(a, n, s);
+        else if (cut.nl == 2) lp_launch<2>(a, n, s);
+        else lp_launch<4>(a, n, s);
         LLM_LAUNCH_CHECK("logprobs_kernel");
     }
     return LLM_OK;
