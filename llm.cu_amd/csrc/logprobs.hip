@@ -28,11 +28,14 @@
 #define LP_MAX_CHUNKS 64       // of a row: one lane each when they are joined
 #define LP_MAX_VOCAB (1 << 20)
 #define LP_SLICE 4096          // rows per launch: a counter each at the front of the workspace
-#define LP_LIST 576            // words of a wavefront's list: a row of 16-byte loads (512 logits), and the k best
+#define LP_LINE 32             // ints from one row's counter to the next: device-scope additions to one line wait for one another
+#define LP_LIST 768            // words of a wavefront's list: a row of 16-byte loads (512 logits) behind what it holds
+#define LP_FEW 3               // lanes above the bound up to which it stays
 #define LP_JOIN (LP_MAX_CHUNKS * LP_MAX_TOP / LP_THREADS) // listed logits per thread when chunks are joined
 #define LP_LOWEST 0x0400u      // order key of -65504, the lowest logit that has a probability
 
 typedef unsigned long long lp_word;
+typedef unsigned long long lp_pair __attribute__((ext_vector_type(2)));
 
 struct LpArgs {
     const half_t *x;
@@ -95,48 +98,80 @@ __device__ __forceinline__ void lp_wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Appends the lanes' words (0: none) to the wavefront's list of n words; returns the new length.
-__device__ __forceinline__ int lp_append(lp_word *list, int n, lp_word w) {
-    const unsigned long long who = __builtin_amdgcn_ballot_w64(w != 0ull);
+// Appends the words of the lanes in `who` (mine: this lane is one) to the wavefront's list of n words; returns the new length.
+__device__ __forceinline__ int lp_append(lp_word *list, int n, unsigned long long who, bool mine, lp_word w) {
     const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
-    if (w) list[n + before] = w;
+    if (mine) list[n + before] = w;
     return n + __popcll(who);
 }
 
-// The k largest of a wavefront's n <= LP_LIST distinct words to the front of its list, largest first, zeros behind the last.
+// How many of list[0 .. n8) are above a and above b: n8 is a multiple of eight (zeros fill the list up), eight words in flight.
+__device__ __forceinline__ void lp_ranks(const lp_word *list, int n8, lp_word a, lp_word b, int &ra, int &rb) {
+    for (int j = 0; j < n8; j += 8) {
+        lp_pair w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const lp_pair *>(list + j + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ra += (w[i][0] > a) + (w[i][1] > a);
+            rb += (w[i][0] > b) + (w[i][1] > b);
+        }
+    }
+}
+
+// The k largest of a wavefront's n <= LP_LIST distinct words to the front of its list, largest first, zeros behind them
+// up to LP_MAX_TOP words.
 __device__ __forceinline__ void lp_cut(lp_word *list, int n, int k) {
     const int lane = threadIdx.x % 64;
-    lp_wave_sync();
+    lp_word w[LP_LIST / 64];
+    auto spread = [&]() __attribute__((always_inline)) { // the list over the lanes
+        lp_wave_sync();
+        lp_word top = 0ull;
+#pragma unroll
+        for (int i = 0; i < LP_LIST / 64; ++i) {
+            w[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0ull;
+            top = w[i] > top ? w[i] : top;
+        }
+        lp_wave_sync();
+        return top;
+    };
+    if (n > 64) { // only what is not below the k-th largest of the lanes' largest: little more than k words, but for equal logits
+        const uint32_t from = lp_kth_key(lp_word_key(spread()), k);
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < LP_LIST / 64; ++i) {
+            const bool mine = w[i] != 0ull && lp_word_key(w[i]) >= from;
+            const unsigned long long who = __builtin_amdgcn_ballot_w64(mine);
+            if (who) n = lp_append(list, n, who, mine, w[i]);
+        }
+    }
     if (n <= 128) {
+        if (lane < 8) list[n + lane] = 0ull;
+        lp_wave_sync();
         const lp_word a = lane < n ? list[lane] : 0ull, b = lane + 64 < n ? list[lane + 64] : 0ull;
         int ra = 0, rb = 0;
-        for (int j = 0; j < n; ++j) {
-            const lp_word w = list[j];
-            ra += w > a;
-            rb += w > b;
-        }
+        lp_ranks(list, (n + 7) & ~7, a, b, ra, rb);
         lp_wave_sync();
         if (a && ra < k) list[ra] = a;
         if (b && rb < k) list[rb] = b;
     } else { // their maximum, k times
-        lp_word w[LP_LIST / 64];
-#pragma unroll
-        for (int i = 0; i < LP_LIST / 64; ++i) w[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0ull;
-        lp_wave_sync();
+        lp_word top = spread();
         for (int r = 0; r < k; ++r) {
-            lp_word top = 0ull;
-#pragma unroll
-            for (int i = 0; i < LP_LIST / 64; ++i) top = w[i] > top ? w[i] : top;
             for (int o = 32; o; o >>= 1) {
                 const lp_word q = __shfl_xor(top, o);
                 top = q > top ? q : top;
             }
-#pragma unroll
-            for (int i = 0; i < LP_LIST / 64; ++i) w[i] = w[i] == top ? 0ull : w[i];
             if (lane == 0) list[r] = top;
+            lp_word rest = 0ull;
+#pragma unroll
+            for (int i = 0; i < LP_LIST / 64; ++i) {
+                w[i] = w[i] == top ? 0ull : w[i];
+                rest = w[i] > rest ? w[i] : rest;
+            }
+            top = rest;
         }
     }
-    if (lane >= n && lane < k) list[lane] = 0ull;
+    if (lane >= (n < k ? n : k) && lane < LP_MAX_TOP) list[lane] = 0ull;
     lp_wave_sync();
 }
 
@@ -147,9 +182,9 @@ __device__ __forceinline__ void lp_join_waves(const lp_word *lists, int k, lp_wo
     __syncthreads();
     if (tid < LP_WAVES * k) {
         const lp_word mine = lists[tid / k * LP_LIST + tid % k];
-        int rank = 0;
-        for (int w = 0; w < LP_WAVES; ++w)
-            for (int j = 0; j < k; ++j) rank += lists[w * LP_LIST + j] > mine;
+        int rank = 0, none = 0;
+#pragma unroll
+        for (int w = 0; w < LP_WAVES; ++w) lp_ranks(lists + w * LP_LIST, (k + 7) & ~7, mine, ~0ull, rank, none);
         if (mine && rank < k) best[rank] = mine;
     }
     __syncthreads();
@@ -159,7 +194,7 @@ __device__ __forceinline__ void lp_join_waves(const lp_word *lists, int k, lp_wo
 template <int NL>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     constexpr int SEG = 64 * 8 * NL;
-    extern __shared__ lp_word lists[]; // LP_WAVES lists of LP_LIST words when k > 0
+    extern __shared__ __attribute__((aligned(16))) lp_word lists[]; // LP_WAVES lists of LP_LIST words when k > 0
     __shared__ lp_word best[LP_MAX_TOP];
     __shared__ float part[LP_WAVES][3];
     __shared__ int is_last;
@@ -170,23 +205,34 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     const half_t ninf = __builtin_bit_cast(half_t, (uint16_t)0xfc00u);
     lp_word *list = lists + wave * LP_LIST;
 
+    // the given tokens' logits, asked for in front of everything else (only the workgroup that ends the row uses them)
+    int id = -1;
+    half_t given = ninf;
+    if (tid < a.n_ids) {
+        id = a.ids[row * a.n_ids + tid];
+        if (id >= 0 && id < a.vocab) given = x[id];
+    }
     // ---- 1. the wavefront's segments: wave, wave + LP_WAVES, ... of the chunk ---------------------------------------------
     const int begin = chunk * a.chunk_len, end = begin + a.chunk_len < a.vocab ? begin + a.chunk_len : a.vocab;
     LpStats st = {-INFINITY, 0.f, 0.f}; // m of the wavefront, sums of the lane
     half_t lane_best = ninf;
-    uint32_t bound = LP_LOWEST; // order key from which on a logit is listed
+    uint32_t bound = LP_LOWEST; // order key from which on a logit is listed, and its value
+    half_t from = lp_value(bound);
     int n = 0;
     half8_t v[NL], next[NL];
-    auto load = [&](half8_t (&d)[NL], int s0) __attribute__((always_inline)) { // -inf behind the end
+    auto load = [&](half8_t (&d)[NL], int s0) __attribute__((always_inline)) {
+        if (s0 + SEG <= end) {
 #pragma unroll
-        for (int u = 0; u < NL; ++u) {
+            for (int u = 0; u < NL; ++u) d[u] = lp_load8(x + s0 + (u * 64 + lane) * 8);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < NL; ++u) { // the chunk's last segment: -inf behind the end
             const int i = s0 + (u * 64 + lane) * 8;
-            if (i + 8 <= end) {
-                d[u] = lp_load8(x + i);
-            } else {
-#pragma unroll
+            d[u] = half8_t{ninf, ninf, ninf, ninf, ninf, ninf, ninf, ninf};
+            if (i + 8 <= end) d[u] = lp_load8(x + i);
+            else if (i < end)
                 for (int e = 0; e < 8; ++e) d[u][e] = i + e < end ? x[i + e] : ninf;
-            }
         }
     };
     int s0 = begin + wave * SEG;
@@ -194,12 +240,14 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     for (; s0 < end; s0 += LP_WAVES * SEG) {
         const bool more = s0 + LP_WAVES * SEG < end;
         if (more) load(next, s0 + LP_WAVES * SEG);
-        half8_t m8 = v[0];
+        half_t lane_max[NL], top = ninf; // a NaN loses against any number here; the sums find it
 #pragma unroll
-        for (int u = 1; u < NL; ++u) m8 = __builtin_elementwise_max(m8, v[u]);
-        half_t top = ninf; // a NaN loses against any number here; the sums find it
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = m8[e] > top ? m8[e] : top;
+        for (int u = 0; u < NL; ++u) {
+            const half4_t m4 = __builtin_elementwise_max(__builtin_shufflevector(v[u], v[u], 0, 1, 2, 3), __builtin_shufflevector(v[u], v[u], 4, 5, 6, 7));
+            const half2_t m2 = __builtin_elementwise_max(__builtin_shufflevector(m4, m4, 0, 1), __builtin_shufflevector(m4, m4, 2, 3));
+            lane_max[u] = m2[0] > m2[1] || m2[1] != m2[1] ? m2[0] : m2[1];
+            top = lane_max[u] > top ? lane_max[u] : top;
+        }
         if (__builtin_amdgcn_ballot_w64((float)top > st.m)) st = lp_rebase(st, fmaxf(st.m, wave_max((float)top)), c);
         const float ref = lp_ref(st.m, c);
 #pragma unroll
@@ -210,29 +258,34 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
                 st.s += p;
                 st.t = fmaf(fmaxf(y, -FLT_MAX), p, st.t); // -inf times zero is zero here; a NaN is in p already
             }
-        if (k > 0 && __builtin_amdgcn_ballot_w64(top >= lp_value(bound))) {
-            lane_best = top > lane_best ? top : lane_best;
-            const uint32_t kth = lp_kth_key(lane_best == ninf ? 0u : lp_key(lane_best), k);
-            bound = kth > bound ? kth : bound;
-            half_t from = lp_value(bound);
+        lane_best = top > lane_best ? top : lane_best;
+        const int lanes = k > 0 ? __popcll(__builtin_amdgcn_ballot_w64(top >= from)) : 0;
+        if (lanes) {
+            if (k == 1 || lanes > LP_FEW) { // the lanes' maxima have moved enough for the bound to follow
+                const uint32_t kth = k == 1 ? lp_key((half_t)st.m) : lp_kth_key(lane_best == ninf ? 0u : lp_key(lane_best), k);
+                bound = kth > bound ? kth : bound;
+                from = lp_value(bound);
+            }
+            uint32_t some = 0u; // loads with a logit from the bound on
 #pragma unroll
-            for (int u = 0; u < NL; ++u) {
-                int count = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) count += __popcll(__builtin_amdgcn_ballot_w64(v[u][e] >= from));
-                if (count == 0) continue;
-                if (n + count > LP_LIST) {
+            for (int u = 0; u < NL; ++u) some |= __builtin_amdgcn_ballot_w64(lane_max[u] >= from) ? 1u << u : 0u;
+            for (int u = 0; some; ++u, some >>= 1) {
+                if (!(some & 1u)) continue;
+                if (n > LP_LIST - 512) {
                     lp_cut(list, n, k);
-                    n = n < k ? n : k;
-                    if (n == k) { // an equal logit further back is not among the k best
-                        const uint32_t above = lp_word_key(list[k - 1]) + 1u;
-                        bound = above > bound ? above : bound;
-                        from = lp_value(bound);
-                    }
+                    n = k;
+                    const uint32_t above = lp_word_key(list[k - 1]) + 1u; // an equal logit further back is not among the k best
+                    bound = above > bound ? above : bound;
+                    from = lp_value(bound);
                 }
+                half8_t w = v[0];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    n = lp_append(list, n, v[u][e] >= from ? lp_make(v[u][e], s0 + (u * 64 + lane) * 8 + e) : 0ull);
+                for (int i = 1; i < NL; ++i) w = i == u ? v[i] : w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const unsigned long long who = __builtin_amdgcn_ballot_w64(w[e] >= from);
+                    if (who) n = lp_append(list, n, who, w[e] >= from, lp_make(w[e], s0 + (u * 64 + lane) * 8 + e));
+                }
             }
         }
         if (more)
@@ -270,10 +323,17 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         if (tid < k) lp_put(a.listed + at * k + tid, best[tid]);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (tid == 0) is_last = __hip_atomic_fetch_add(a.counters + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+        if (tid == 0) is_last = __hip_atomic_fetch_add(a.counters + row * LP_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
         __syncthreads();
         if (!is_last) return;
-        if (tid == 0) a.counters[row] = 0; // ready for the next launch
+        if (tid == 0) a.counters[row * LP_LINE] = 0; // ready for the next launch
+        lp_word w[LP_JOIN]; // all of what the chunks left is asked for at once
+        const lp_word *listed = a.listed + row * a.chunks * k;
+#pragma unroll
+        for (int j = 0; j < LP_JOIN; ++j) {
+            const int q = tid + LP_THREADS * j;
+            w[j] = q < a.chunks * k ? lp_get(listed + q) : 0ull;
+        }
         float mine[3] = {-INFINITY, 0.f, 0.f};
         if (lane < a.chunks)
 #pragma unroll
@@ -281,20 +341,13 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         M = wave_max(mine[0]);
         const LpStats p = lp_rebase({mine[0], mine[1], mine[2]}, M, c);
         st = {M, wave_sum(p.s), wave_sum(p.t)};
-        if (k > 0) { // the chunks' lists, with a bound as above
-            const lp_word *listed = a.listed + row * a.chunks * k;
-            const int total = a.chunks * k;
-            lp_word w[LP_JOIN], top = 0ull;
-#pragma unroll
-            for (int j = 0; j < LP_JOIN; ++j) {
-                const int q = tid + LP_THREADS * j;
-                w[j] = q < total ? lp_get(listed + q) : 0ull;
-                top = w[j] > top ? w[j] : top;
-            }
-            const uint32_t kth = lp_kth_key(lp_word_key(top), k);
+        if (k > 0) {
             n = 0;
 #pragma unroll
-            for (int j = 0; j < LP_JOIN; ++j) n = lp_append(list, n, lp_word_key(w[j]) >= kth ? w[j] : 0ull);
+            for (int j = 0; j < LP_JOIN; ++j) {
+                const unsigned long long who = __builtin_amdgcn_ballot_w64(w[j] != 0ull);
+                if (who) n = lp_append(list, n, who, w[j] != 0ull, w[j]);
+            }
             lp_cut(list, n, k);
             __syncthreads();
             lp_join_waves(lists, k, best);
@@ -307,9 +360,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     const float log_s = none ? 0.f : logf(st.s) - off * 0.693147180559945309f;
     if (tid == 0) a.entropy[row] = invalid ? NAN : log_s - mean;
     if (tid < a.n_ids) {
-        const int id = a.ids[row * a.n_ids + tid];
         float lp = NAN;
-        if (id >= 0 && id < a.vocab && !invalid) lp = ((float)x[id] - m0) * a.inv_t - log_s;
+        if (id >= 0 && id < a.vocab && !invalid) lp = ((float)given - m0) * a.inv_t - log_s;
         a.logprob[row * a.n_ids + tid] = lp;
     }
     if (tid < k) {
@@ -325,7 +377,7 @@ struct LpCut {
     int nl, chunk_len, chunks;
 };
 static LpCut lp_cut_row(int rows, int vocab) {
-    const int target = 2048; // workgroups
+    const int target = 256; // workgroups
     int want = (target + rows - 1) / rows;
     if (want > LP_MAX_CHUNKS) want = LP_MAX_CHUNKS;
     int len = (vocab + want - 1) / want;
@@ -346,9 +398,9 @@ extern "C" {
 
 // counters of LP_SLICE rows, then the statistics and lists of one launch
 size_t llm_logprobs_workspace_bytes(int rows, int vocab, int k) {
-    if (rows < 1 || vocab < 1 || vocab > LP_MAX_VOCAB || k < 0) return sizeof(int) * LP_SLICE;
+    if (rows < 1 || vocab < 1 || vocab > LP_MAX_VOCAB || k < 0) return sizeof(int) * LP_SLICE * LP_LINE;
     const size_t n = (size_t)(rows < LP_SLICE ? rows : LP_SLICE) * lp_cut_row(rows, vocab).chunks;
-    return sizeof(int) * LP_SLICE + n * (sizeof(uint32_t) * 4 + sizeof(lp_word) * k);
+    return sizeof(int) * LP_SLICE * LP_LINE + n * (sizeof(uint32_t) * 4 + sizeof(lp_word) * k);
 }
 
 int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temperature, const int32_t *ids, int n_ids,
@@ -373,7 +425,7 @@ int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temp
     a.chunk_len = cut.chunk_len;
     a.inv_t = 1.f / temperature;
     a.counters = (int *)workspace;
-    a.stats = (uint32_t *)workspace + LP_SLICE;
+    a.stats = (uint32_t *)workspace + LP_SLICE * LP_LINE;
     hipStream_t s = (hipStream_t)stream;
     for (int r0 = 0; r0 < rows; r0 += LP_SLICE) {
         const int n = rows - r0 < LP_SLICE ? rows - r0 : LP_SLICE;
