@@ -7,6 +7,7 @@
 // holds position row0 + r), position p_z is the new token, whose rotated key and value are appended to the own cache.
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -67,50 +68,79 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 // that the bank swizzle assigns to its slot.  The four wavefronts of a workgroup are QT query tiles x KG groups of keys x DH
 // parts of the output dims (DH = 2: both compute the scores, each half of the output).
 // ---------------------------------------------------------------------------------------------------------------
-#define AS_WAVES 4
+#define AS_WAVES 8
 #define AS_THREADS (64 * AS_WAVES)
 #define AS_LDS_PTR(p) ((__attribute__((address_space(3))) void *)(p))
+#define AS_GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void *)(p))
 
 template <int HD, int QT> struct AsShape {
-    static constexpr int KG = QT == 4 ? 1 : QT == 2 ? 2 : HD >= 64 ? 2 : 4;
+    static constexpr int SK = HD >= 128 ? 64 : HD >= 64 ? 128 : 256; // keys per stage: 32 KB
+    static constexpr int KG = SK / 32 < AS_WAVES / QT ? SK / 32 : AS_WAVES / QT;
     static constexpr int DH = AS_WAVES / (QT * KG);
-    static constexpr int SK = HD >= 64 ? 64 : 128;       // keys per stage
     static constexpr int NCH = SK / 32 / KG;             // chunks of a stage per wavefront
     static constexpr int TILE = SK * HD;                 // halves of a K or V^T tile
-    static constexpr int NS = HD >= 128 ? 2 : 4;         // stages of the ring
+    static constexpr int NS = 4;                         // stages of the ring
     static constexpr int DT = HD / 32 / DH;              // 32-dim tiles of the output per wavefront
     static_assert(QT * KG * DH == AS_WAVES && NCH >= 1 && DT >= 1, "roles of the wavefronts");
 };
 template <int HD> constexpr int as_lds_halves() { return AsShape<HD, 1>::NS * 2 * AsShape<HD, 1>::TILE; }
 
-// Spans of a launch, the same for every KV head.
-struct AsSpans {
-    int span;          // keys, a multiple of 128
-    int n_prefix;      // spans of the longest prefix the launch is sized for
-    int n_tail;        // spans of the longest tail, per sequence
-    float *acc, *ml;   // [prefix: kvh][span][batch * G], then [tails: z][kvh][span][G] rows of HD (acc) and 2 (ml) floats
+// Who does what.  The rows of a KV head -- the prefix, then each sequence's own rows -- form one line of units of 32 keys, an
+// empty unit in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the line,
+// whatever the lengths are.  A workgroup leaves one part for each piece of the line that its share touches: part i of the
+// prefix comes from workgroup i, and workgroup i's part of tail z goes to place i + z (both only grow along the line).
+#define AS_UNIT 32
+#define AS_START 8
+struct AsPlan {
+    int wgs, min_share; // workgroups per KV head; units a share has at least
+    float *acc, *ml;    // [kvh][wgs][batch * G] of the prefix, then [kvh][wgs + batch][G] of the tails: rows of HD (acc), 2 (ml)
 };
+struct AsLine {
+    int prefix_units, share, prefix, own_first, lead; // own_first: own row of the first position behind the prefix; lead: rows in
+                                                      // front of it in the aligned eight that it lies in
+    int tail, first, units;                           // lane z: own rows of sequence z, its first unit, its units
+};
+// Every lane of a wavefront calls it; lane z looks at sequence z.
+template <bool DEV> __device__ __forceinline__ AsLine as_line(const SharedArgs &a, int batch, int wgs, int min_share) {
+    const int lane = threadIdx.x % 64;
+    const SharedSeq s = shared_seq<DEV>(a, lane < batch ? lane : 0);
+    AsLine ln;
+    ln.prefix = __builtin_amdgcn_readfirstlane(s.prefix);
+    ln.own_first = __builtin_amdgcn_readfirstlane(s.first);
+    ln.lead = ln.own_first & 7;
+    ln.prefix_units = (ln.prefix + AS_UNIT - 1) / AS_UNIT;
+    ln.tail = lane < batch ? s.tail : 0;
+    ln.units = ln.tail > 0 ? (ln.lead + ln.tail + AS_UNIT - 1) / AS_UNIT : 0;
+    int end = ln.units > 0 ? ln.units + AS_START : 0; // inclusive sums over the sequences
+#pragma unroll
+    for (int o = 1; o < LLM_MAX_BATCH; o <<= 1) {
+        const int q = __shfl_up(end, o);
+        if (lane >= o) end += q;
+    }
+    ln.first = ln.prefix_units + end - ln.units;
+    const int total = ln.prefix_units + __builtin_amdgcn_readlane(end, LLM_MAX_BATCH - 1);
+    ln.share = (total + wgs - 1) / wgs;
+    if (ln.share < min_share) ln.share = min_share;
+    return ln;
+}
 
-// Rows of one span: chunks of eight rows from `begin` on, of which lo .. hi - 1 count.
+// Rows of one part: tiles from `begin` (a multiple of eight) on, of which rows lo .. hi - 1 count.
 struct AsRange {
     int begin, lo, hi;
 };
-__device__ __forceinline__ AsRange as_prefix_range(const SharedSeq &s, const AsSpans &sp, int i) {
-    const int b = i * sp.span, e = b + sp.span;
-    return {b, b, e < s.prefix ? e : s.prefix};
-}
-__device__ __forceinline__ AsRange as_tail_range(const SharedSeq &s, const AsSpans &sp, int i) {
-    const int b = (s.first & ~7) + i * sp.span, e = b + sp.span, end = s.first + s.tail;
-    return {b, b > s.first ? b : s.first, e < end ? e : end};
-}
 
-template <int HD, int QT, class QueryRow>
+// q_row(r): query row r of the tiles, not rotated (any r below 32 QT); q_seq(r): its row of the (cos, sin) table's rows that
+// are staged, cs_row(i), i < LLM_MAX_BATCH.
+template <int HD, int QT, class QRow, class QSeq, class CsRow>
 __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const half_t *vbase, const int max_pos, const AsRange r,
-                                        const int rows, QueryRow query, float *acc, float *ml) {
+                                        const int rows, QRow q_row, QSeq q_seq, CsRow cs_row, float *acc, float *ml) {
     using S = AsShape<HD, QT>;
     constexpr int SK = S::SK, KG = S::KG, DH = S::DH, NS = S::NS, DT = S::DT, TILE = S::TILE;
-    constexpr int NC = HD / 8, NCV = SK / 8;                     // 16-byte chunks per K row / V^T row of a tile
+    constexpr int NC = HD / 8, NCV = SK / 8, NCC = HD / 4;       // 16-byte chunks per K row / V^T row of a tile / row of the table
     constexpr int LPW = TILE * 2 / 1024 / AS_WAVES;              // loads per wavefront, stage and tile (1 KB each)
+    constexpr int Q_HALVES = 32 * QT * HD, CS_HALVES = LLM_MAX_BATCH * HD * 2;
+    constexpr int NQ = Q_HALVES + CS_HALVES <= 2 * TILE ? 1 : 2; // last slots of the ring that hold queries and table rows first
+    static_assert(Q_HALVES + CS_HALVES <= NQ * 2 * TILE && NQ < NS, "room for the queries");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     const int qt = wave % QT, kg = wave / QT % KG, dh = wave / (QT * KG);
     const int n = lane % 32, hb = lane / 32;
@@ -119,7 +149,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
     // ---- loads: instruction i of a wavefront covers rows 4 i + wave, in units of the rows that 1 KB holds ----
     const __amdgpu_buffer_rsrc_t rs_k = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, 0, max_pos * HD * 2, 0x00020000);
     const __amdgpu_buffer_rsrc_t rs_v = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, 0, HD * max_pos * 2, 0x00020000);
-    auto swz = [](int row, int chunks) { return row / (16 / chunks) & (chunks - 1); };
+    auto swz = [](int row, int chunks) { return chunks >= 16 ? row & 15 : row / (16 / chunks) & (chunks - 1); }; // of 16-byte chunks over the banks
     const int krow = wave * (64 / NC) + lane / NC, vrow = wave * (64 / NCV) + lane / NCV;
     const int kchunk = lane % NC ^ swz(krow, NC), vchunk = lane % NCV ^ swz(vrow, NCV);
     const uint32_t koff = (uint32_t)krow * (HD * 2) + (uint32_t)kchunk * 16;
@@ -127,7 +157,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
     auto issue = [&](int slot, int st) __attribute__((always_inline)) { // stage st into slot % NS of the ring
         half_t *buf = smem + slot % NS * 2 * TILE;
         const int key = r.begin + st * SK;
-        if (key + SK <= max_pos) {
+        if (key + SK <= r.hi) {
 #pragma unroll
             for (int i = 0; i < LPW; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * AS_WAVES + wave) * 512), 16, koff,
@@ -138,13 +168,13 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
                                                          (uint32_t)key * 2 + (uint32_t)i * (AS_WAVES * (64 / NCV)) * (uint32_t)max_pos * 2u, 0, 0);
             return;
         }
-        // the tile reaches past the cache's last row: the rows behind it are read from the last ones (and masked later)
-        const int vkey = key + 8 * vchunk < max_pos - 8 ? key + 8 * vchunk : max_pos - 8;
+        // the tile reaches past the last row that counts: what lies behind is read from that one (and masked later)
+        const int vkey = key + 8 * vchunk < r.hi ? key + 8 * vchunk : (r.hi - 1) & ~7;
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
             const int row = key + i * AS_WAVES * (64 / NC) + krow;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * AS_WAVES + wave) * 512), 16,
-                                                     (uint32_t)(row < max_pos ? row : max_pos - 1) * (HD * 2) + (uint32_t)kchunk * 16, 0, 0, 0);
+                                                     (uint32_t)(row < r.hi ? row : r.hi - 1) * (HD * 2) + (uint32_t)kchunk * 16, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < LPW; ++i)
@@ -152,29 +182,44 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
                                                      ((uint32_t)(i * AS_WAVES * (64 / NCV) + vrow) * (uint32_t)max_pos + (uint32_t)vkey) * 2u, 0, 0, 0);
     };
 
-    // ---- queries: lane (n, hb) holds dims 16 ks + 8 hb .. + 7 of row 32 qt + n; rotated while the first tiles travel ----
-    half8_t qf[HD / 16];
-    float4_t cs[HD / 16][2];
-    {
-        const float *table;
-        const half_t *q = query(32 * qt + n < rows ? 32 * qt + n : rows - 1, &table);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-            qf[ks] = load8(q + 16 * ks + 8 * hb);
-            cs[ks][0] = *reinterpret_cast<const float4_t *>(table + 16 * ks + 8 * hb);
-            cs[ks][1] = *reinterpret_cast<const float4_t *>(table + 16 * ks + 8 * hb + 4);
-        }
+    // ---- queries and the (cos, sin) rows of their positions: through the last slots of the ring, like the tiles and in front
+    // of them, so that no load into registers is waited for behind the tiles' (loads complete in order: that would be a wait
+    // for the whole ring) ----
+    half_t *q_l = smem + (NS - NQ) * 2 * TILE, *cs_l = q_l + Q_HALVES;
+    for (int i = wave; i < Q_HALVES / 512; i += AS_WAVES) { // 1 KB: 64 / NC rows, swizzled like a K tile
+        const int row = i * (64 / NC) + lane / NC;
+        __builtin_amdgcn_global_load_lds(AS_GLOBAL_PTR(q_row(row) + (lane % NC ^ swz(row, NC)) * 8), AS_LDS_PTR(q_l + i * 512), 16, 0, 0);
     }
-    // always NS stages (a short span's last one more than once): the number of loads in flight is known everywhere
+    for (int i = wave; i < CS_HALVES / 512; i += AS_WAVES) {
+        const int row = i * (64 / NCC) + lane / NCC;
+        __builtin_amdgcn_global_load_lds(AS_GLOBAL_PTR(cs_row(row) + (lane % NCC ^ (row & (NCC - 1) & 15)) * 4), AS_LDS_PTR(cs_l + i * 512), 16, 0, 0);
+    }
+    // always NS stages (a short piece's last one more than once): the number of loads in flight is known everywhere
     const int issued = stages > NS ? stages : NS;
 #pragma unroll
-    for (int st = 0; st < NS; ++st) issue(st, st < stages ? st : stages - 1);
+    for (int st = 0; st < NS - NQ; ++st) issue(st, st < stages ? st : stages - 1);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - NQ) * 2 * LPW) : "memory");
+    half8_t qf[HD / 16]; // lane (n, hb) holds dims 16 ks + 8 hb .. + 7 of row 32 qt + n
+    {
+        const int row = 32 * qt + n, z = q_seq(row);
+        float4_t cs[HD / 16][2];
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-        float c[8];
+        for (int ks = 0; ks < HD / 16; ++ks) {
+            qf[ks] = load8(q_l + row * HD + ((2 * ks + hb) ^ swz(row, NC)) * 8);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = cs[ks][i / 4][i % 4];
-        qf[ks] = rope_rotate8(qf[ks], c);
+            for (int i = 0; i < 2; ++i)
+                cs[ks][i] = *reinterpret_cast<const float4_t *>(cs_l + z * HD * 2 + ((4 * ks + 2 * hb + i) ^ (z & (NCC - 1) & 15)) * 8);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); // every wavefront has its queries: the slots are free
+#pragma unroll
+        for (int st = NS - NQ; st < NS; ++st) issue(st, st < stages ? st : stages - 1);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) { // rotated while the tiles travel
+            float c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = cs[ks][i / 4][i % 4];
+            qf[ks] = rope_rotate8(qf[ks], c);
+        }
     }
 
     float16_t o[DT];
@@ -198,12 +243,25 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
         else if (behind == 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LPW) : "memory");
         else if (behind == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * LPW) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(6 * LPW) : "memory");
-        const half_t *ks_ = smem + st % NS * 2 * TILE, *vs_ = ks_ + TILE;
+        half_t *ks_ = smem + st % NS * 2 * TILE, *vs_ = ks_ + TILE;
+        const int key_st = r.begin + st * SK;
+        const bool edge = key_st < r.lo || key_st + SK > r.hi;
+        if (edge) { // values outside the piece's rows may be anything, NaN included: zero in the tile
+            for (int i = tid; i < HD * NCV; i += AS_THREADS) {
+                const int dim = i / NCV, c = i % NCV, k0 = key_st + 8 * c;
+                if (k0 >= r.lo && k0 + 8 <= r.hi) continue;
+                half_t *at = vs_ + dim * SK + (c ^ swz(dim, NCV)) * 8;
+                half8_t v = load8(at);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = k0 + e >= r.lo && k0 + e < r.hi ? v[e] : (half_t)0.f;
+                store8(at, v);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
 #pragma unroll
         for (int j = 0; j < S::NCH; ++j) {
-            const int kc = 32 * (kg + KG * j), key0 = r.begin + st * SK + kc; // the chunk in the stage; its first key
-            if (key0 >= r.hi || key0 + 32 <= r.lo) continue;                  // no key of the span (the same for every lane)
-            const bool edge = key0 < r.lo || key0 + 32 > r.hi;
+            const int kc = 32 * (kg + KG * j), key0 = key_st + kc;   // the chunk in the stage; its first key
+            if (key0 >= r.hi || key0 + 32 <= r.lo) continue;        // no key of the piece (the same for every lane)
             float16_t s;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = 0.f;
@@ -250,14 +308,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const int dim = 32 * (dh * DT + t) + n;
-                    half8_t vf = load8(vs_ + dim * SK + ((kc / 8 + 2 * u + hb) ^ swz(dim, NCV)) * 8);
-                    if (edge) { // rows outside the span may hold anything
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int key = key0 + 16 * u + 8 * hb + e;
-                            vf[e] = key >= r.lo && key < r.hi ? vf[e] : (half_t)0.f;
-                        }
-                    }
+                    const half8_t vf = load8(vs_ + dim * SK + ((kc / 8 + 2 * u + hb) ^ swz(dim, NCV)) * 8);
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[u], o[t], 0, 0, 0);
                 }
             }
@@ -318,142 +369,149 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
     }
 }
 
-// Grid: (prefix spans, then tail spans of every sequence) x KV heads, the KV head fastest: consecutive workgroups go round the
-// XCDs, so that a head's queries and tables stay in one XCD's L2.
+// Grid: wgs x KV heads, the KV head fastest: consecutive workgroups go round the XCDs, so that a head's queries and tables stay
+// in one XCD's L2.  The arguments in front of `a` are in registers when the kernel starts.
 template <int HD, int G, int QT, bool DEV>
-__global__ __launch_bounds__(AS_THREADS, 2) void attn_shared_part_kernel(const SharedArgs a, const AsSpans sp) {
+__global__ __launch_bounds__(AS_THREADS) void attn_shared_part_kernel(float *acc, float *ml, const half_t *qkv, const float *table, int n_kv_heads,
+                                                                      int batch, int wgs, int min_share, int ldq, int prefix_max,
+                                                                      const SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) half_t smem[];
-    const int kvh = blockIdx.x % a.n_kv_heads, task = blockIdx.x / a.n_kv_heads;
-    const int rows = a.batch * G;
-    if (task < sp.n_prefix) {
-        const SharedSeq s = shared_seq<DEV>(a, 0);
-        const AsRange r = as_prefix_range(s, sp, task);
-        if (r.lo >= r.hi) return;
-        const size_t at = ((size_t)kvh * sp.n_prefix + task) * rows;
-        auto query = [&](int row, const float **cs) {
-            const int z = row / G;
-            const SharedSeq sz = shared_seq<DEV>(a, z);
-            *cs = a.table + (size_t)(sz.prefix + sz.tail) * HD;
-            return a.qkv + (size_t)z * a.ldq + (size_t)(kvh * G + row % G) * HD;
+    const int kvh = blockIdx.x % n_kv_heads, wg = blockIdx.x / n_kv_heads;
+    const int rows = batch * G;
+    const SharedSeq s0 = shared_seq<DEV>(a, 0); // asked for next to the positions that the line needs
+    const AsLine ln = as_line<DEV>(a, batch, wgs, min_share);
+    const int from = wg * ln.share, to = from + ln.share; // this workgroup's units
+    if (from < ln.prefix_units) {
+        const int end = to * AS_UNIT < ln.prefix ? to * AS_UNIT : ln.prefix;
+        const size_t at = ((size_t)kvh * wgs + wg) * rows;
+        auto q_row = [&](int row) {
+            row = row < rows ? row : rows - 1;
+            return qkv + (size_t)(row / G) * ldq + (size_t)(kvh * G + row % G) * HD;
         };
-        as_span<HD, QT>(smem, s.kp + (size_t)kvh * a.prefix_max * HD, s.vp + (size_t)kvh * HD * a.prefix_max, a.prefix_max, r, rows, query,
-                        sp.acc + at * HD, sp.ml + at * 2);
-    } else {
-        const int z = (task - sp.n_prefix) % a.batch, i = (task - sp.n_prefix) / a.batch;
+        auto q_seq = [&](int row) { return row < rows ? row / G : batch - 1; };
+        auto cs_row = [&](int z) { return table + (size_t)(ln.prefix + __shfl(ln.tail, z)) * HD; };
+        as_span<HD, QT>(smem, s0.kp + (size_t)kvh * prefix_max * HD, s0.vp + (size_t)kvh * HD * prefix_max, prefix_max,
+                        AsRange{from * AS_UNIT, from * AS_UNIT, end}, rows, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
+    }
+    unsigned long long mine = __builtin_amdgcn_ballot_w64(ln.units > 0 && ln.first < to && ln.first + ln.units > from); // tails
+    for (; mine; mine &= mine - 1) {
+        const int z = __builtin_ctzll(mine);
+        const int first = __builtin_amdgcn_readlane(ln.first, z), u = __builtin_amdgcn_readlane(ln.units, z), tail = __builtin_amdgcn_readlane(ln.tail, z);
+        const int u0 = from > first ? from - first : 0, u1 = to - first < u ? to - first : u;
+        const int base = ln.own_first - ln.lead, b = base + u0 * AS_UNIT, e = base + u1 * AS_UNIT, end = ln.own_first + tail;
+        const size_t at = (size_t)n_kv_heads * wgs * rows + ((size_t)kvh * (wgs + batch) + wg + z) * G;
         const SharedSeq s = shared_seq<DEV>(a, z);
-        const AsRange r = as_tail_range(s, sp, i);
-        if (r.lo >= r.hi) return;
-        const size_t at = (size_t)a.n_kv_heads * sp.n_prefix * rows + (((size_t)z * a.n_kv_heads + kvh) * sp.n_tail + i) * G;
-        auto query = [&](int row, const float **cs) {
-            *cs = a.table + (size_t)(s.prefix + s.tail) * HD;
-            return a.qkv + (size_t)z * a.ldq + (size_t)(kvh * G + row) * HD;
-        };
-        as_span<HD, 1>(smem, s.kc + (size_t)kvh * a.max_pos * HD, s.vc + (size_t)kvh * HD * a.max_pos, a.max_pos, r, G, query, sp.acc + at * HD,
-                       sp.ml + at * 2);
+        auto q_row = [&](int row) { return qkv + (size_t)z * ldq + (size_t)(kvh * G + (row < G ? row : G - 1)) * HD; };
+        auto q_seq = [&](int) { return 0; };
+        auto cs_row = [&](int) { return table + (size_t)(ln.prefix + tail) * HD; };
+        __syncthreads(); // the LDS of the piece before
+        as_span<HD, 1>(smem, s.kc + (size_t)kvh * a.max_pos * HD, s.vc + (size_t)kvh * HD * a.max_pos, a.max_pos,
+                       AsRange{b, b > ln.own_first ? b : ln.own_first, e < end ? e : end}, G, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
     }
 }
 
-// One workgroup per query head and sequence: the new token's score, the spans' weights, the weighted sum; the first head of a
-// group appends the new key and value.
+// One workgroup per query head and sequence: the parts' weights (first wavefront) and the new token's score (second one) while
+// the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.
 #define AS_MERGE_THREADS 256
+#define AS_MERGE_AHEAD 8
 template <int HD, int G, bool DEV>
-__global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(const SharedArgs a, const AsSpans sp) {
+__global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(const float *acc, const float *ml, const half_t *qkv, const float *table,
+                                                                             int n_kv_heads, int batch, int wgs, int min_share, int ldq, int max_pos,
+                                                                             const SharedArgs a) {
     constexpr int LPR = HD / 4, GROUPS = AS_MERGE_THREADS / LPR; // lanes per row of HD floats, rows side by side
-    extern __shared__ float weight[]; // one per span
-    __shared__ float l_all, w_new;
+    extern __shared__ float weight[]; // one per part
+    __shared__ float m_parts, l_parts, m_new;
     __shared__ float4_t part[GROUPS][LPR];
     const int h = blockIdx.x, z = blockIdx.y, kvh = h / G, g = h % G, tid = threadIdx.x, lane = tid % 64;
-    const int rows = a.batch * G, Hq = a.n_kv_heads * G;
+    const int rows = batch * G, Hq = n_kv_heads * G;
     const SharedSeq s = shared_seq<DEV>(a, z);
     const int pos = s.prefix + s.tail, row = s.first + s.tail;
-    const int np = (s.prefix + sp.span - 1) / sp.span, nt = s.tail > 0 ? ((s.first & 7) + s.tail + sp.span - 1) / sp.span : 0, ns = np + nt;
-    const size_t pre = (size_t)kvh * sp.n_prefix * rows + (size_t)z * G + g;
-    const size_t own = (size_t)a.n_kv_heads * sp.n_prefix * rows + ((size_t)z * a.n_kv_heads + kvh) * sp.n_tail * G + g;
+    const AsLine ln = as_line<DEV>(a, batch, wgs, min_share);
+    const int first = __builtin_amdgcn_readlane(ln.first, z), u = __builtin_amdgcn_readlane(ln.units, z);
+    const int np = (ln.prefix_units + ln.share - 1) / ln.share;
+    const int w0 = first / ln.share, nt = u > 0 ? (first + u - 1) / ln.share - w0 + 1 : 0, ns = np + nt;
+    const size_t pre = (size_t)kvh * wgs * rows + (size_t)z * G + g;
+    const size_t own = (size_t)n_kv_heads * wgs * rows + ((size_t)kvh * (wgs + batch) + w0 + z) * G + g;
     auto slot = [&](int i) { return i < np ? pre + (size_t)i * rows : own + (size_t)(i - np) * G; };
-    const half_t *line = a.qkv + (size_t)z * a.ldq;
-    const half_t *vn = line + (size_t)(Hq + a.n_kv_heads + kvh) * HD;
+    const half_t *line = qkv + (size_t)z * ldq;
+    const half_t *vn = line + (size_t)(Hq + n_kv_heads + kvh) * HD;
+    const int d4 = tid % LPR, grp = tid / LPR;
+    float4_t v[AS_MERGE_AHEAD];
+#pragma unroll
+    for (int j = 0; j < AS_MERGE_AHEAD; ++j) {
+        v[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (grp + GROUPS * j < ns) v[j] = *reinterpret_cast<const float4_t *>(acc + slot(grp + GROUPS * j) * HD + 4 * d4);
+    }
     if (tid < 64) {
-        // the new token: eight dims per lane
+        float M = -FLT_MAX, l = 0.f;
+        for (int i = lane; i < ns; i += 64) {
+            const float2_t p = *reinterpret_cast<const float2_t *>(ml + 2 * slot(i));
+            // relative to this lane's largest so far
+            const float m = fmaxf(M, p[0]);
+            l = l * __builtin_amdgcn_exp2f(M - m) + p[1] * __builtin_amdgcn_exp2f(p[0] - m);
+            M = m;
+            weight[i] = p[0];
+        }
+        const float all = wave_max(M);
+        l = wave_sum(l * __builtin_amdgcn_exp2f(M - all));
+        for (int i = lane; i < ns; i += 64) weight[i] = __builtin_amdgcn_exp2f(weight[i] - all);
+        if (lane == 0) {
+            m_parts = all;
+            l_parts = l;
+        }
+    } else if (tid < 128) {
         float dot = 0.f;
-        if (lane < HD / 8) {
-            const float *cs = a.table + (size_t)pos * HD + lane * 8;
+        if (lane < HD / 8) { // eight dims per lane
+            const float *cs = table + (size_t)pos * HD + lane * 8;
             const half8_t q = rope_rotate8(load8(line + (size_t)h * HD + lane * 8), cs);
             const half8_t k = rope_rotate8(load8(line + (size_t)(Hq + kvh) * HD + lane * 8), cs);
             dot = dot8(q, k, 0.f);
             if (g == 0) {
-                store8(s.kc + ((size_t)kvh * a.max_pos + row) * HD + lane * 8, k);
-                const half8_t v = load8(vn + lane * 8);
+                store8(s.kc + ((size_t)kvh * max_pos + row) * HD + lane * 8, k);
+                const half8_t vv = load8(vn + lane * 8);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s.vc[((size_t)kvh * HD + lane * 8 + e) * a.max_pos + row] = v[e];
+                for (int e = 0; e < 8; ++e) s.vc[((size_t)kvh * HD + lane * 8 + e) * max_pos + row] = vv[e];
             }
         }
-        const float m_new = wave_sum(dot) * (1.44269504088896341f / sqrtf((float)HD));
-        float M = m_new;
-        for (int i = lane; i < ns; i += 64) {
-            const float m = sp.ml[2 * slot(i)];
-            weight[i] = m;
-            M = fmaxf(M, m);
-        }
-        M = wave_max(M);
-        float l = 0.f;
-        for (int i = lane; i < ns; i += 64) {
-            const float w = __builtin_amdgcn_exp2f(weight[i] - M);
-            weight[i] = w;
-            l += w * sp.ml[2 * slot(i) + 1];
-        }
-        l = wave_sum(l);
-        if (lane == 0) {
-            w_new = __builtin_amdgcn_exp2f(m_new - M);
-            l_all = l + w_new;
-        }
+        dot = wave_sum(dot) * (1.44269504088896341f / sqrtf((float)HD));
+        if (lane == 0) m_new = dot;
     }
     __syncthreads();
-    const int d4 = tid % LPR, grp = tid / LPR;
     float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = grp; i < ns; i += GROUPS) {
-        const float4_t v = *reinterpret_cast<const float4_t *>(sp.acc + slot(i) * HD + 4 * d4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += weight[i] * v[e];
+    for (int j = 0; j < AS_MERGE_AHEAD; ++j) {
+        if (grp + GROUPS * j < ns) {
+            const float w = weight[grp + GROUPS * j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += w * v[j][e];
+        }
+    }
+    for (int i = grp + GROUPS * AS_MERGE_AHEAD; i < ns; i += GROUPS) {
+        const float4_t x = *reinterpret_cast<const float4_t *>(acc + slot(i) * HD + 4 * d4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += weight[i] * x[e];
     }
     part[grp][d4] = o;
     __syncthreads();
     if (tid < LPR) {
-        const half4_t v = *reinterpret_cast<const half4_t *>(vn + 4 * d4);
+        const float M = fmaxf(m_parts, m_new), f = __builtin_amdgcn_exp2f(m_parts - M), w = __builtin_amdgcn_exp2f(m_new - M);
+        const float inv = 1.0f / (f * l_parts + w);
+        const half4_t x = *reinterpret_cast<const half4_t *>(vn + 4 * d4);
+        half_t *out = a.out + (size_t)z * a.ldo + (size_t)h * HD + 4 * d4;
+        o = part[0][d4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = w_new * (float)v[e];
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i)
+        for (int i = 1; i < GROUPS; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] += part[i][d4][e];
-        half_t *out = a.out + (size_t)z * a.ldo + (size_t)h * HD + 4 * d4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = (half_t)(o[e] / l_all);
+        for (int e = 0; e < 4; ++e) out[e] = (half_t)((f * o[e] + w * (float)x[e]) * inv);
     }
 }
 
-// Spans per KV head, all sequences together: two workgroups on each of the 256 compute units, but enough for the prefix next to
-// one span for each sequence's own rows.
-static int as_target(int n_kv_heads, int batch) {
-    const int fill = n_kv_heads < 512 ? 512 / n_kv_heads : 1;
-    return fill > 2 * batch ? fill : 2 * batch;
-}
+// Workgroups per KV head: one on each of the 256 compute units.
+static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 ? 256 / n_kv_heads : 1; }
 
-static AsSpans as_spans(const SharedArgs &a) {
-    AsSpans sp = {};
-    const long long target = as_target(a.n_kv_heads, a.batch), total = a.max_prefix + (long long)a.batch * a.max_tail;
-    for (long long span = (total / target + 127) / 128 * 128;; span += 128) {
-        if (span == 0) continue;
-        const long long np = (a.max_prefix + span - 1) / span, nt = a.max_tail > 0 ? (a.max_tail + 7 + span - 1) / span : 0;
-        if (np + a.batch * nt <= target) { // holds at the latest where both are one
-            sp.span = (int)span;
-            sp.n_prefix = (int)np;
-            sp.n_tail = (int)nt;
-            return sp;
-        }
-    }
-}
-
-template <int HD, int G, int QT, bool DEV> static int launch_shared(const SharedArgs &a, AsSpans sp, hipStream_t s) {
+template <int HD, int G, int QT, bool DEV> static int launch_shared(const SharedArgs &a, const AsPlan &pl, hipStream_t s) {
     const size_t smem = sizeof(half_t) * as_lds_halves<HD>();
     auto kern = attn_shared_part_kernel<HD, G, QT, DEV>;
     static std::atomic<uint64_t> attr_done{0};
@@ -461,27 +519,34 @@ template <int HD, int G, int QT, bool DEV> static int launch_shared(const Shared
         int rc = llm_ensure_max_smem((const void *)kern, smem, attr_done);
         if (rc != LLM_OK) return rc;
     }
-    const int tasks = sp.n_prefix + a.batch * sp.n_tail;
-    if (tasks > 0) {
-        kern<<<dim3((unsigned)tasks * a.n_kv_heads), dim3(AS_THREADS), smem, s>>>(a, sp);
+    // no more workgroups than the longest lengths of the launch give shares to
+    const long long units = (a.max_prefix + AS_UNIT - 1) / AS_UNIT +
+                            (a.max_tail > 0 ? (long long)a.batch * ((a.max_tail + 7 + AS_UNIT - 1) / AS_UNIT + AS_START) : 0);
+    long long used = (units + pl.min_share - 1) / pl.min_share;
+    if (used > pl.wgs) used = pl.wgs;
+    if (used > 0) {
+        kern<<<dim3((unsigned)used * a.n_kv_heads), dim3(AS_THREADS), smem, s>>>(pl.acc, pl.ml, a.qkv, a.table, a.n_kv_heads, a.batch, pl.wgs,
+                                                                                   pl.min_share, a.ldq, a.prefix_max, a);
         LLM_LAUNCH_CHECK("attn_shared_part_kernel");
     }
-    attn_shared_merge_kernel<HD, G, DEV><<<dim3(a.n_kv_heads * G, a.batch), dim3(AS_MERGE_THREADS),
-                                           sizeof(float) * (sp.n_prefix + sp.n_tail + 1), s>>>(a, sp);
+    attn_shared_merge_kernel<HD, G, DEV><<<dim3(a.n_kv_heads * G, a.batch), dim3(AS_MERGE_THREADS), sizeof(float) * 2 * (pl.wgs + 1), s>>>(
+        pl.acc, pl.ml, a.qkv, a.table, a.n_kv_heads, a.batch, pl.wgs, pl.min_share, a.ldq, a.max_pos, a);
     LLM_LAUNCH_CHECK("attn_shared_merge_kernel");
     return LLM_OK;
 }
 
 template <int HD, int G> static int launch_shared(const SharedArgs &a, void *ws, hipStream_t s) {
-    AsSpans sp = as_spans(a);
     const int rows = a.batch * G;
-    sp.acc = (float *)ws;
-    sp.ml = sp.acc + ((size_t)a.n_kv_heads * sp.n_prefix * rows + (size_t)a.batch * a.n_kv_heads * sp.n_tail * G) * HD;
+    AsPlan pl = {};
+    pl.wgs = as_wgs(a.n_kv_heads);
+    pl.min_share = 4;
+    pl.acc = (float *)ws;
+    pl.ml = pl.acc + (size_t)a.n_kv_heads * ((size_t)pl.wgs * rows + (size_t)(pl.wgs + a.batch) * G) * HD;
     constexpr int MAXR = G * LLM_MAX_BATCH;
     // as many query tiles as the batch fills
-    if (rows <= 32 || MAXR <= 32) return a.desc ? launch_shared<HD, G, 1, true>(a, sp, s) : launch_shared<HD, G, 1, false>(a, sp, s);
-    if (rows <= 64 || MAXR <= 64) return a.desc ? launch_shared<HD, G, MAXR >= 64 ? 2 : 1, true>(a, sp, s) : launch_shared<HD, G, MAXR >= 64 ? 2 : 1, false>(a, sp, s);
-    return a.desc ? launch_shared<HD, G, MAXR >= 128 ? 4 : 1, true>(a, sp, s) : launch_shared<HD, G, MAXR >= 128 ? 4 : 1, false>(a, sp, s);
+    if (rows <= 32 || MAXR <= 32) return a.desc ? launch_shared<HD, G, 1, true>(a, pl, s) : launch_shared<HD, G, 1, false>(a, pl, s);
+    if (rows <= 64 || MAXR <= 64) return a.desc ? launch_shared<HD, G, MAXR >= 64 ? 2 : 1, true>(a, pl, s) : launch_shared<HD, G, MAXR >= 64 ? 2 : 1, false>(a, pl, s);
+    return a.desc ? launch_shared<HD, G, MAXR >= 128 ? 4 : 1, true>(a, pl, s) : launch_shared<HD, G, MAXR >= 128 ? 4 : 1, false>(a, pl, s);
 }
 
 static int dispatch_shared(const char *name, const SharedArgs &a, int n_heads, int head_dim, void *ws, hipStream_t s) {
@@ -525,9 +590,8 @@ extern "C" {
 
 size_t llm_attn_shared_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int batch) {
     if (n_heads < 1 || n_kv_heads < 1 || head_dim < 1 || batch < 1) return 16;
-    // at most as_target spans of the prefix, with batch rows per head, and as many of the tails
-    const size_t target = (size_t)as_target(n_kv_heads, batch);
-    return sizeof(float) * n_heads * target * (batch + 1) * (head_dim + 2);
+    const size_t wgs = (size_t)as_wgs(n_kv_heads);
+    return sizeof(float) * n_heads * (wgs * batch + wgs + batch) * (head_dim + 2);
 }
 
 int llm_attn_decode_rope_shared(const uint16_t *qkv, int ldq, const uint16_t *k_prefix, const uint16_t *v_prefix, int prefix_len,
