@@ -68,29 +68,31 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 // that the bank swizzle assigns to its slot.  The four wavefronts of a workgroup are QT query tiles x KG groups of keys x DH
 // parts of the output dims (DH = 2: both compute the scores, each half of the output).
 // ---------------------------------------------------------------------------------------------------------------
-#define AS_WAVES 8
+#define AS_WAVES 4
 #define AS_THREADS (64 * AS_WAVES)
+#define AS_RING 2     // stages, of 32 KB at most
+#define AS_PER_CU 2   // workgroups that a compute unit holds
 #define AS_LDS_PTR(p) ((__attribute__((address_space(3))) void *)(p))
 #define AS_GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void *)(p))
 
 template <int HD, int QT> struct AsShape {
-    static constexpr int SK = HD >= 128 ? 64 : HD >= 64 ? 128 : 256; // keys per stage: 32 KB
+    static constexpr int SK = HD >= 128 ? 64 : 128;      // keys per stage
     static constexpr int KG = SK / 32 < AS_WAVES / QT ? SK / 32 : AS_WAVES / QT;
     static constexpr int DH = AS_WAVES / (QT * KG);
     static constexpr int NCH = SK / 32 / KG;             // chunks of a stage per wavefront
     static constexpr int TILE = SK * HD;                 // halves of a K or V^T tile
-    static constexpr int NS = 4;                         // stages of the ring
+    static constexpr int NS = AS_RING;                   // stages of the ring
     static constexpr int DT = HD / 32 / DH;              // 32-dim tiles of the output per wavefront
     static_assert(QT * KG * DH == AS_WAVES && NCH >= 1 && DT >= 1, "roles of the wavefronts");
 };
 template <int HD> constexpr int as_lds_halves() { return AsShape<HD, 1>::NS * 2 * AsShape<HD, 1>::TILE; }
 
-// Who does what.  The rows of a KV head -- the prefix, then each sequence's own rows -- form one line of units of 32 keys, an
-// empty unit in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the line,
+// Who does what.  The rows of a KV head -- the prefix, then each sequence's own rows -- form one line of units of 64 keys, with
+// AS_START empty units in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the line,
 // whatever the lengths are.  A workgroup leaves one part for each piece of the line that its share touches: part i of the
 // prefix comes from workgroup i, and workgroup i's part of tail z goes to place i + z (both only grow along the line).
-#define AS_UNIT 32
-#define AS_START 8
+#define AS_UNIT 64
+#define AS_START 3
 struct AsPlan {
     int wgs, min_share; // workgroups per KV head; units a share has at least
     float *acc, *ml;    // [kvh][wgs][batch * G] of the prefix, then [kvh][wgs + batch][G] of the tails: rows of HD (acc), 2 (ml)
@@ -140,7 +142,8 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
     constexpr int LPW = TILE * 2 / 1024 / AS_WAVES;              // loads per wavefront, stage and tile (1 KB each)
     constexpr int Q_HALVES = 32 * QT * HD, CS_HALVES = LLM_MAX_BATCH * HD * 2;
     constexpr int NQ = Q_HALVES + CS_HALVES <= 2 * TILE ? 1 : 2; // last slots of the ring that hold queries and table rows first
-    static_assert(Q_HALVES + CS_HALVES <= NQ * 2 * TILE && NQ < NS, "room for the queries");
+    static_assert(AS_WAVES * (64 / NC) % 16 == 0 && AS_WAVES * (64 / NCV) % 16 == 0, "the swizzle is the same for all loads of a lane");
+    static_assert(Q_HALVES + CS_HALVES <= NQ * 2 * TILE && NQ <= NS, "room for the queries");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     const int qt = wave % QT, kg = wave / QT % KG, dh = wave / (QT * KG);
     const int n = lane % 32, hb = lane / 32;
@@ -372,7 +375,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
 // Grid: wgs x KV heads, the KV head fastest: consecutive workgroups go round the XCDs, so that a head's queries and tables stay
 // in one XCD's L2.  The arguments in front of `a` are in registers when the kernel starts.
 template <int HD, int G, int QT, bool DEV>
-__global__ __launch_bounds__(AS_THREADS) void attn_shared_part_kernel(float *acc, float *ml, const half_t *qkv, const float *table, int n_kv_heads,
+__global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_shared_part_kernel(float *acc, float *ml, const half_t *qkv, const float *table, int n_kv_heads,
                                                                       int batch, int wgs, int min_share, int ldq, int prefix_max,
                                                                       const SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) half_t smem[];
@@ -509,7 +512,7 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
 }
 
 // Workgroups per KV head: one on each of the 256 compute units.
-static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 ? 256 / n_kv_heads : 1; }
+static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 * AS_PER_CU ? 256 * AS_PER_CU / n_kv_heads : 1; }
 
 template <int HD, int G, int QT, bool DEV> static int launch_shared(const SharedArgs &a, const AsPlan &pl, hipStream_t s) {
     const size_t smem = sizeof(half_t) * as_lds_halves<HD>();
@@ -539,7 +542,7 @@ template <int HD, int G> static int launch_shared(const SharedArgs &a, void *ws,
     const int rows = a.batch * G;
     AsPlan pl = {};
     pl.wgs = as_wgs(a.n_kv_heads);
-    pl.min_share = 4;
+    pl.min_share = 2;
     pl.acc = (float *)ws;
     pl.ml = pl.acc + (size_t)a.n_kv_heads * ((size_t)pl.wgs * rows + (size_t)(pl.wgs + a.batch) * G) * HD;
     constexpr int MAXR = G * LLM_MAX_BATCH;
