@@ -68,24 +68,32 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 // that the bank swizzle assigns to its slot.  The four wavefronts of a workgroup are QT query tiles x KG groups of keys x DH
 // parts of the output dims (DH = 2: both compute the scores, each half of the output).
 // ---------------------------------------------------------------------------------------------------------------
-#define AS_WAVES 4
+#define AS_WAVES 4    // wavefronts of a workgroup
 #define AS_THREADS (64 * AS_WAVES)
-#define AS_RING 2     // stages, of 32 KB at most
+#define AS_RING 2     // stages
 #define AS_PER_CU 2   // workgroups that a compute unit holds
 #define AS_LDS_PTR(p) ((__attribute__((address_space(3))) void *)(p))
 #define AS_GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void *)(p))
 
-template <int HD, int QT> struct AsShape {
-    static constexpr int SK = HD >= 128 ? 64 : 128;      // keys per stage
-    static constexpr int KG = SK / 32 < AS_WAVES / QT ? SK / 32 : AS_WAVES / QT;
-    static constexpr int DH = AS_WAVES / (QT * KG);
+template <int HD, int QT, int W> struct AsShape { // W wavefronts
+    static constexpr int SK = (HD >= 128 ? 16 : 32) * W; // keys per stage
+    static constexpr int KG = SK / 32 < W / QT ? SK / 32 : W / QT;
+    static constexpr int DH = W / (QT * KG);
     static constexpr int NCH = SK / 32 / KG;             // chunks of a stage per wavefront
     static constexpr int TILE = SK * HD;                 // halves of a K or V^T tile
     static constexpr int NS = AS_RING;                   // stages of the ring
     static constexpr int DT = HD / 32 / DH;              // 32-dim tiles of the output per wavefront
-    static_assert(QT * KG * DH == AS_WAVES && NCH >= 1 && DT >= 1, "roles of the wavefronts");
+    static_assert(QT * KG * DH == W && NCH >= 1 && DT >= 1, "roles of the wavefronts");
 };
-template <int HD> constexpr int as_lds_halves() { return AsShape<HD, 1>::NS * 2 * AsShape<HD, 1>::TILE; }
+// LDS: the ring, and in its place at the end what the wavefronts hold: four accumulators of every lane form a block, lane (n, hb)
+// at n + 40 hb of its 73 places of 16 bytes, so that neither a block nor a query row's dims in order meet on the banks.
+#define AS_BLOCK 73
+#define AS_HALF 40
+template <int HD, int QT, int W> constexpr int as_held() { return 4 * AsShape<HD, QT, W>::DT * AS_BLOCK * 4 + 128; } // floats of a wavefront
+template <int HD, int QT, int W> constexpr int as_lds_bytes() {
+    constexpr int ring = AsShape<HD, QT, W>::NS * 4 * AsShape<HD, QT, W>::TILE, held = W * as_held<HD, QT, W>() * 4;
+    return ring > held ? ring : held;
+}
 
 // Who does what.  The rows of a KV head -- the prefix, then each sequence's own rows -- form one line of units of 64 keys, with
 // AS_START empty units in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the line,
@@ -126,74 +134,85 @@ template <bool DEV> __device__ __forceinline__ AsLine as_line(const SharedArgs &
     return ln;
 }
 
-// Rows of one part: tiles from `begin` (a multiple of eight) on, of which rows lo .. hi - 1 count.
-struct AsRange {
-    int begin, lo, hi;
+// A piece of the line: rows of one head's half-caches, in tiles from `begin` (a multiple of eight) on, of which lo .. hi - 1 count.
+struct AsPiece {
+    const half_t *k, *v;
+    int max_pos, begin, lo, hi;
 };
 
-// q_row(r): query row r of the tiles, not rotated (any r below 32 QT); q_seq(r): its row of the (cos, sin) table's rows that
-// are staged, cs_row(i), i < LLM_MAX_BATCH.
-template <int HD, int QT, class QRow, class QSeq, class CsRow>
-__device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const half_t *vbase, const int max_pos, const AsRange r,
-                                        const int rows, QRow q_row, QSeq q_seq, CsRow cs_row, float *acc, float *ml) {
-    using S = AsShape<HD, QT>;
+// The tiles of NP pieces, one behind the other, for up to 32 QT query rows.
+// q_row(r): query row r, not rotated (any r below 32 QT); q_seq(r): which of the staged rows cs_row(i), i < LLM_MAX_BATCH, of the
+// (cos, sin) table is its position's.
+// between(qf): called when the rotated query rows are there, lane (n, hb) holding dims 16 ks + 8 hb .. + 7 of row 32 qt + n;
+// what it leaves in LDS outside the ring is visible behind as_tiles.
+// Leaves every wavefront's output, maxima and sums in the LDS, behind a barrier, for as_result.
+template <int HD, int QT, int W, int NP, class QRow, class QSeq, class CsRow, class Between>
+__device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], QRow q_row, QSeq q_seq, CsRow cs_row, Between between) {
+    using S = AsShape<HD, QT, W>;
     constexpr int SK = S::SK, KG = S::KG, DH = S::DH, NS = S::NS, DT = S::DT, TILE = S::TILE;
     constexpr int NC = HD / 8, NCV = SK / 8, NCC = HD / 4;       // 16-byte chunks per K row / V^T row of a tile / row of the table
-    constexpr int LPW = TILE * 2 / 1024 / AS_WAVES;              // loads per wavefront, stage and tile (1 KB each)
+    constexpr int LPW = TILE * 2 / 1024 / W;                     // loads per wavefront, stage and tile (1 KB each)
     constexpr int Q_HALVES = 32 * QT * HD, CS_HALVES = LLM_MAX_BATCH * HD * 2;
     constexpr int NQ = Q_HALVES + CS_HALVES <= 2 * TILE ? 1 : 2; // last slots of the ring that hold queries and table rows first
-    static_assert(AS_WAVES * (64 / NC) % 16 == 0 && AS_WAVES * (64 / NCV) % 16 == 0, "the swizzle is the same for all loads of a lane");
+    static_assert(W * (64 / NC) % 16 == 0 && W * (64 / NCV) % 16 == 0, "the swizzle is the same for all loads of a lane");
     static_assert(Q_HALVES + CS_HALVES <= NQ * 2 * TILE && NQ <= NS, "room for the queries");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     const int qt = wave % QT, kg = wave / QT % KG, dh = wave / (QT * KG);
     const int n = lane % 32, hb = lane / 32;
-    const int stages = (r.hi - r.begin + SK - 1) / SK;
+    const int stages_0 = (pc[0].hi - pc[0].begin + SK - 1) / SK; // of the first piece
+    const int real = NP == 1 ? stages_0 : stages_0 + (pc[NP - 1].hi - pc[NP - 1].begin + SK - 1) / SK;
+    const int stages = real > 0 ? real : 1;                      // no row at all: one tile that is masked throughout
 
-    // ---- loads: instruction i of a wavefront covers rows 4 i + wave, in units of the rows that 1 KB holds ----
-    const __amdgpu_buffer_rsrc_t rs_k = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, 0, max_pos * HD * 2, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rs_v = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, 0, HD * max_pos * 2, 0x00020000);
+    // ---- loads: instruction i of a wavefront covers rows W i + wave, in units of the rows that 1 KB holds ----
     auto swz = [](int row, int chunks) { return chunks >= 16 ? row & 15 : row / (16 / chunks) & (chunks - 1); }; // of 16-byte chunks over the banks
     const int krow = wave * (64 / NC) + lane / NC, vrow = wave * (64 / NCV) + lane / NCV;
     const int kchunk = lane % NC ^ swz(krow, NC), vchunk = lane % NCV ^ swz(vrow, NCV);
     const uint32_t koff = (uint32_t)krow * (HD * 2) + (uint32_t)kchunk * 16;
-    const uint32_t voff = (uint32_t)vrow * (uint32_t)max_pos * 2u + (uint32_t)vchunk * 16;
-    auto issue = [&](int slot, int st) __attribute__((always_inline)) { // stage st into slot % NS of the ring
+    auto first_key = [&](int st, const AsPiece &p) { return NP > 1 && &p != &pc[0] ? p.begin + (st - stages_0) * SK : p.begin + st * SK; };
+    auto issue_of = [&](int slot, int st, const AsPiece &p) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rs_k = __builtin_amdgcn_make_buffer_rsrc((void *)p.k, 0, p.max_pos * HD * 2, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rs_v = __builtin_amdgcn_make_buffer_rsrc((void *)p.v, 0, HD * p.max_pos * 2, 0x00020000);
         half_t *buf = smem + slot % NS * 2 * TILE;
-        const int key = r.begin + st * SK;
-        if (key + SK <= r.hi) {
+        const int key = first_key(st, p), hi = p.hi > 0 ? p.hi : 1;
+        if (key + SK <= hi) {
+            const uint32_t voff = (uint32_t)vrow * (uint32_t)p.max_pos * 2u + (uint32_t)vchunk * 16;
 #pragma unroll
             for (int i = 0; i < LPW; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * AS_WAVES + wave) * 512), 16, koff,
-                                                         (uint32_t)key * (HD * 2) + (uint32_t)i * (AS_WAVES * 1024), 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * W + wave) * 512), 16, koff,
+                                                         (uint32_t)key * (HD * 2) + (uint32_t)i * (W * 1024), 0, 0);
 #pragma unroll
             for (int i = 0; i < LPW; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_v, AS_LDS_PTR(buf + TILE + (i * AS_WAVES + wave) * 512), 16, voff,
-                                                         (uint32_t)key * 2 + (uint32_t)i * (AS_WAVES * (64 / NCV)) * (uint32_t)max_pos * 2u, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_v, AS_LDS_PTR(buf + TILE + (i * W + wave) * 512), 16, voff,
+                                                         (uint32_t)key * 2 + (uint32_t)i * (W * (64 / NCV)) * (uint32_t)p.max_pos * 2u, 0, 0);
             return;
         }
         // the tile reaches past the last row that counts: what lies behind is read from that one (and masked later)
-        const int vkey = key + 8 * vchunk < r.hi ? key + 8 * vchunk : (r.hi - 1) & ~7;
+        const int vkey = key + 8 * vchunk < hi ? key + 8 * vchunk : (hi - 1) & ~7;
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
-            const int row = key + i * AS_WAVES * (64 / NC) + krow;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * AS_WAVES + wave) * 512), 16,
-                                                     (uint32_t)(row < r.hi ? row : r.hi - 1) * (HD * 2) + (uint32_t)kchunk * 16, 0, 0, 0);
+            const int row = key + i * W * (64 / NC) + krow;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_k, AS_LDS_PTR(buf + (i * W + wave) * 512), 16,
+                                                     (uint32_t)(row < hi ? row : hi - 1) * (HD * 2) + (uint32_t)kchunk * 16, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < LPW; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_v, AS_LDS_PTR(buf + TILE + (i * AS_WAVES + wave) * 512), 16,
-                                                     ((uint32_t)(i * AS_WAVES * (64 / NCV) + vrow) * (uint32_t)max_pos + (uint32_t)vkey) * 2u, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_v, AS_LDS_PTR(buf + TILE + (i * W + wave) * 512), 16,
+                                                     ((uint32_t)(i * W * (64 / NCV) + vrow) * (uint32_t)p.max_pos + (uint32_t)vkey) * 2u, 0, 0, 0);
+    };
+    auto issue = [&](int slot, int st) __attribute__((always_inline)) { // stage st into slot % NS of the ring
+        if (NP == 1 || st < stages_0) issue_of(slot, st, pc[0]);
+        else issue_of(slot, st, pc[NP - 1]);
     };
 
     // ---- queries and the (cos, sin) rows of their positions: through the last slots of the ring, like the tiles and in front
     // of them, so that no load into registers is waited for behind the tiles' (loads complete in order: that would be a wait
     // for the whole ring) ----
     half_t *q_l = smem + (NS - NQ) * 2 * TILE, *cs_l = q_l + Q_HALVES;
-    for (int i = wave; i < Q_HALVES / 512; i += AS_WAVES) { // 1 KB: 64 / NC rows, swizzled like a K tile
+    for (int i = wave; i < Q_HALVES / 512; i += W) { // 1 KB: 64 / NC rows, swizzled like a K tile
         const int row = i * (64 / NC) + lane / NC;
         __builtin_amdgcn_global_load_lds(AS_GLOBAL_PTR(q_row(row) + (lane % NC ^ swz(row, NC)) * 8), AS_LDS_PTR(q_l + i * 512), 16, 0, 0);
     }
-    for (int i = wave; i < CS_HALVES / 512; i += AS_WAVES) {
+    for (int i = wave; i < CS_HALVES / 512; i += W) {
         const int row = i * (64 / NCC) + lane / NCC;
         __builtin_amdgcn_global_load_lds(AS_GLOBAL_PTR(cs_row(row) + (lane % NCC ^ (row & (NCC - 1) & 15)) * 4), AS_LDS_PTR(cs_l + i * 512), 16, 0, 0);
     }
@@ -202,8 +221,8 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
 #pragma unroll
     for (int st = 0; st < NS - NQ; ++st) issue(st, st < stages ? st : stages - 1);
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - NQ) * 2 * LPW) : "memory");
-    half8_t qf[HD / 16]; // lane (n, hb) holds dims 16 ks + 8 hb .. + 7 of row 32 qt + n
-    {
+    half8_t qf[HD / 16];
+    { // lane (n, hb) takes dims 16 ks + 8 hb .. + 7 of row 32 qt + n
         const int row = 32 * qt + n, z = q_seq(row);
         float4_t cs[HD / 16][2];
 #pragma unroll
@@ -224,6 +243,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
             qf[ks] = rope_rotate8(qf[ks], c);
         }
     }
+    between(qf);
 
     float16_t o[DT];
 #pragma unroll
@@ -247,16 +267,23 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
         else if (behind == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * LPW) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(6 * LPW) : "memory");
         half_t *ks_ = smem + st % NS * 2 * TILE, *vs_ = ks_ + TILE;
-        const int key_st = r.begin + st * SK;
-        const bool edge = key_st < r.lo || key_st + SK > r.hi;
-        if (edge) { // values outside the piece's rows may be anything, NaN included: zero in the tile
-            for (int i = tid; i < HD * NCV; i += AS_THREADS) {
-                const int dim = i / NCV, c = i % NCV, k0 = key_st + 8 * c;
-                if (k0 >= r.lo && k0 + 8 <= r.hi) continue;
-                half_t *at = vs_ + dim * SK + (c ^ swz(dim, NCV)) * 8;
+        const bool second = NP > 1 && st >= stages_0;
+        const int key_st = second ? first_key(st, pc[NP - 1]) : first_key(st, pc[0]);
+        const int r_lo = second ? pc[NP - 1].lo : pc[0].lo, r_hi = second ? pc[NP - 1].hi : pc[0].hi;
+        // Chunks of 32 keys that the piece begins or ends in: values outside its rows may be anything, NaN included, and
+        // become zero in the tile (scores are masked below).
+        const int cut_lo = key_st < r_lo ? (r_lo - key_st) & ~31 : SK, cut_hi = key_st + SK > r_hi ? (r_hi - key_st) & ~31 : SK;
+        const bool lo_cut = cut_lo < SK && ((r_lo - key_st) & 31), hi_cut = cut_hi < SK && ((r_hi - key_st) & 31);
+        if (lo_cut || hi_cut) {
+            for (int i = tid; i < HD * 8; i += 64 * W) { // four 16-byte pieces of a dim's row in each of the two chunks
+                const int dim = i / 8, at_hi = i / 4 % 2, k0 = (at_hi ? cut_hi : cut_lo) + 8 * (i % 4);
+                if (!(at_hi ? hi_cut : lo_cut) || (at_hi && lo_cut && cut_hi == cut_lo)) continue;
+                const int f = r_lo - key_st - k0, l = r_hi - key_st - k0; // elements f .. l - 1 stay
+                if (f <= 0 && l >= 8) continue;
+                half_t *at = vs_ + dim * SK + (k0 / 8 ^ swz(dim, NCV)) * 8;
                 half8_t v = load8(at);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k0 + e >= r.lo && k0 + e < r.hi ? v[e] : (half_t)0.f;
+                for (int e = 0; e < 8; ++e) v[e] = e >= f && e < l ? v[e] : (half_t)0.f;
                 store8(at, v);
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -264,7 +291,7 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
 #pragma unroll
         for (int j = 0; j < S::NCH; ++j) {
             const int kc = 32 * (kg + KG * j), key0 = key_st + kc;   // the chunk in the stage; its first key
-            if (key0 >= r.hi || key0 + 32 <= r.lo) continue;        // no key of the piece (the same for every lane)
+            if (key0 >= r_hi || key0 + 32 <= r_lo) continue;        // no key of the piece (the same for every lane)
             float16_t s;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = 0.f;
@@ -272,11 +299,11 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(load8(ks_ + krow_l * HD + ((2 * ks + hb) ^ swz(krow_l, NC)) * 8), qf[ks], s, 0, 0, 0);
-            if (edge) {
+            if (key0 < r_lo || key0 + 32 > r_hi) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int key = key0 + 16 * (e / 8) + 8 * hb + e % 8;
-                    s[e] = key >= r.lo && key < r.hi ? s[e] : -FLT_MAX;
+                    s[e] = key >= r_lo && key < r_hi ? s[e] : -FLT_MAX;
                 }
             }
             // The reference of the exponentials moves when a score leaves it behind by 2^8: probabilities stay below 2^8 in
@@ -327,48 +354,59 @@ __device__ __forceinline__ void as_span(half_t *smem, const half_t *kbase, const
         xhalf(l_run, lo, hi);
         l_run = lo + hi;
     }
-    // ---- the groups of keys into one (through the LDS of the ring), then out ----
-    if (KG > 1) {
-        constexpr int PER = 64 * (16 * DT + 2); // floats per wavefront
-        float *ex = reinterpret_cast<float *>(smem);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int slot = qt + QT * dh;
-        if (kg > 0) {
-            float *d = ex + ((kg - 1) * QT * DH + slot) * PER;
+    // ---- into the LDS, in place of the ring ----
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    float *held = reinterpret_cast<float *>(smem) + wave * as_held<HD, QT, W>();
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) d[(16 * t + e) * 64 + lane] = o[t][e];
-            d[16 * DT * 64 + lane] = m_run;
-            d[(16 * DT + 1) * 64 + lane] = l_run;
-        }
-        __syncthreads();
-        if (kg > 0) return;
+        for (int e4 = 0; e4 < 4; ++e4)
+            *reinterpret_cast<float4_t *>(held + ((4 * t + e4) * AS_BLOCK + n + AS_HALF * hb) * 4) =
+                float4_t{o[t][4 * e4], o[t][4 * e4 + 1], o[t][4 * e4 + 2], o[t][4 * e4 + 3]};
+    *reinterpret_cast<float2_t *>(held + 4 * DT * AS_BLOCK * 4 + 2 * lane) = float2_t{m_run, l_run};
+    __syncthreads();
+}
+
+// What as_tiles left for dims 4 d4 .. + 3 of a query row: the groups of keys joined (unnormalised), the row's maximum (base 2)
+// and sum.
+template <int HD, int QT, int W>
+__device__ __forceinline__ float4_t as_result(const half_t *smem, int row, int d4, float &m, float &l) {
+    using S = AsShape<HD, QT, W>;
+    constexpr int PER = as_held<HD, QT, W>();
+    // dim 4 d4 = 32 (dh DT + t) + 8 e4 + 4 hb
+    const int tile = d4 / 8, dh = tile / S::DT, t = tile % S::DT, e4 = d4 / 2 % 4, n = row % 32;
+    const float *base = reinterpret_cast<const float *>(smem) + (row / 32 + QT * S::KG * dh) * PER; // key group 0; the others QT wavefronts apart
+    float2_t ml[S::KG];
+    m = -FLT_MAX;
 #pragma unroll
-        for (int g = 1; g < KG; ++g) {
-            const float *d = ex + ((g - 1) * QT * DH + slot) * PER;
-            const float m2 = d[16 * DT * 64 + lane], l2 = d[(16 * DT + 1) * 64 + lane];
-            const float m_new = fmaxf(m_run, m2), f1 = __builtin_amdgcn_exp2f(m_run - m_new), f2 = __builtin_amdgcn_exp2f(m2 - m_new);
-            l_run = l_run * f1 + l2 * f2;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[t][e] = o[t][e] * f1 + d[(16 * t + e) * 64 + lane] * f2;
-            m_run = m_new;
-        }
+    for (int g = 0; g < S::KG; ++g) {
+        ml[g] = *reinterpret_cast<const float2_t *>(base + g * QT * PER + 4 * S::DT * AS_BLOCK * 4 + 2 * n);
+        m = fmaxf(m, ml[g][0]);
     }
-    const int row = 32 * qt + n;
-    if (row < rows) {
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+    for (int g = 0; g < S::KG; ++g) {
+        const float f = __builtin_amdgcn_exp2f(ml[g][0] - m); // 0 for a group without a key
+        const float4_t x = *reinterpret_cast<const float4_t *>(base + g * QT * PER + ((4 * t + e4) * AS_BLOCK + n + AS_HALF * (d4 % 2)) * 4);
+        l += f * ml[g][1];
 #pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4)
-                *reinterpret_cast<float4_t *>(acc + (size_t)row * HD + 32 * (dh * DT + t) + 8 * e4 + 4 * hb) =
-                    float4_t{o[t][4 * e4], o[t][4 * e4 + 1], o[t][4 * e4 + 2], o[t][4 * e4 + 3]};
-        if (dh == 0 && hb == 0) {
-            ml[2 * row] = m_run;
-            ml[2 * row + 1] = l_run;
-        }
+        for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+    }
+    return o;
+}
+
+// One part of the line, left for the merge.
+template <int HD, int QT, class QRow, class QSeq, class CsRow>
+__device__ __forceinline__ void as_part(half_t *smem, const AsPiece &piece, const int rows, QRow q_row, QSeq q_seq, CsRow cs_row, float *acc,
+                                        float *ml) {
+    const AsPiece pc[1] = {piece};
+    as_tiles<HD, QT, AS_WAVES, 1>(smem, pc, q_row, q_seq, cs_row, [](const half8_t (&)[HD / 16]) {});
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += AS_THREADS) {
+        const int row = i / (HD / 4), d4 = i % (HD / 4);
+        float m, l;
+        *reinterpret_cast<float4_t *>(acc + (size_t)i * 4) = as_result<HD, QT, AS_WAVES>(smem, row, d4, m, l);
+        if (d4 == 0) *reinterpret_cast<float2_t *>(ml + 2 * row) = float2_t{m, l};
     }
 }
 
@@ -393,8 +431,9 @@ __global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_sha
         };
         auto q_seq = [&](int row) { return row < rows ? row / G : batch - 1; };
         auto cs_row = [&](int z) { return table + (size_t)(ln.prefix + __shfl(ln.tail, z)) * HD; };
-        as_span<HD, QT>(smem, s0.kp + (size_t)kvh * prefix_max * HD, s0.vp + (size_t)kvh * HD * prefix_max, prefix_max,
-                        AsRange{from * AS_UNIT, from * AS_UNIT, end}, rows, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
+        as_part<HD, QT>(smem, AsPiece{s0.kp + (size_t)kvh * prefix_max * HD, s0.vp + (size_t)kvh * HD * prefix_max, prefix_max, from * AS_UNIT,
+                                      from * AS_UNIT, end},
+                        rows, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
     }
     unsigned long long mine = __builtin_amdgcn_ballot_w64(ln.units > 0 && ln.first < to && ln.first + ln.units > from); // tails
     for (; mine; mine &= mine - 1) {
@@ -408,15 +447,17 @@ __global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_sha
         auto q_seq = [&](int) { return 0; };
         auto cs_row = [&](int) { return table + (size_t)(ln.prefix + tail) * HD; };
         __syncthreads(); // the LDS of the piece before
-        as_span<HD, 1>(smem, s.kc + (size_t)kvh * a.max_pos * HD, s.vc + (size_t)kvh * HD * a.max_pos, a.max_pos,
-                       AsRange{b, b > ln.own_first ? b : ln.own_first, e < end ? e : end}, G, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
+        as_part<HD, 1>(smem, AsPiece{s.kc + (size_t)kvh * a.max_pos * HD, s.vc + (size_t)kvh * HD * a.max_pos, a.max_pos, b,
+                                     b > ln.own_first ? b : ln.own_first, e < end ? e : end},
+                       G, q_row, q_seq, cs_row, acc + at * HD, ml + at * 2);
     }
 }
 
 // One workgroup per query head and sequence: the parts' weights (first wavefront) and the new token's score (second one) while
 // the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.
 #define AS_MERGE_THREADS 256
-#define AS_MERGE_AHEAD 8
+// parts per thread asked for at once (80 at head size 128, more than a head of eight has)
+#define AS_MERGE_AHEAD 10
 template <int HD, int G, bool DEV>
 __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(const float *acc, const float *ml, const half_t *qkv, const float *table,
                                                                              int n_kv_heads, int batch, int wgs, int min_share, int ldq, int max_pos,
@@ -511,11 +552,69 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
     }
 }
 
-// Workgroups per KV head: one on each of the 256 compute units.
+// Short lengths: one workgroup of eight wavefronts per KV head and sequence goes through the prefix and the sequence's own rows,
+// takes the new token's key with its queries (row G of the query tile: the same position, the same rotation), and writes the
+// result -- one launch, the prefix read once per sequence (from the caches of the chip after the first time).
+#define AS_DIRECT_WAVES 8
+template <int HD, int G, bool DEV>
+__global__ __launch_bounds__(64 * AS_DIRECT_WAVES) void attn_shared_direct_kernel(const half_t *qkv, const float *table, half_t *out, int n_kv_heads,
+                                                                                 int ldq, int ldo, int prefix_max, int max_pos,
+                                                                                 const SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) half_t smem[];
+    __shared__ __attribute__((aligned(16))) half_t k_new[HD], q_rot[G * HD];
+    const int kvh = blockIdx.x, z = blockIdx.y, Hq = n_kv_heads * G, tid = threadIdx.x, lane = tid % 64;
+    const SharedSeq s = shared_seq<DEV>(a, z);
+    const int pos = s.prefix + s.tail;
+    const half_t *line = qkv + (size_t)z * ldq, *vn = line + (size_t)(Hq + n_kv_heads + kvh) * HD;
+    half_t *kc = s.kc + (size_t)kvh * max_pos * HD, *vc = s.vc + (size_t)kvh * HD * max_pos;
+    // dims 4 d4 .. + 3 of head h are this thread's to write (threads beyond the last item: none)
+    const int h = tid / (HD / 4), d4 = tid % (HD / 4);
+    const half4_t v_new = *reinterpret_cast<const half4_t *>(vn + 4 * d4);
+    const AsPiece pc[2] = {{s.kp + (size_t)kvh * prefix_max * HD, s.vp + (size_t)kvh * HD * prefix_max, prefix_max, 0, 0, s.prefix},
+                           {kc, vc, max_pos, s.tail > 0 ? s.first & ~7 : 0, s.tail > 0 ? s.first : 0, s.tail > 0 ? s.first + s.tail : 0}};
+    auto q_row = [&](int row) { return line + (size_t)(row < G ? kvh * G + row : Hq + kvh) * HD; };
+    auto q_seq = [&](int) { return 0; };
+    auto cs_row = [&](int) { return table + (size_t)pos * HD; };
+    as_tiles<HD, 1, AS_DIRECT_WAVES, 2>(smem, pc, q_row, q_seq, cs_row, [&](const half8_t (&qf)[HD / 16]) {
+        const int n = lane % 32, hb = lane / 32;
+        if (tid < 64 && n <= G) {
+            half_t *d = n < G ? q_rot + n * HD : k_new;
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) store8(d + 16 * ks + 8 * hb, qf[ks]);
+        }
+    });
+    static_assert(G * (HD / 4) <= 64 * AS_DIRECT_WAVES, "one item per thread");
+    if (tid < G * (HD / 4)) {
+        float m, l, dot = 0.f;
+        const float4_t o = as_result<HD, 1, AS_DIRECT_WAVES>(smem, h, d4, m, l);
+        // the score of the new token: HD / 4 lanes share a head, each a part of the dims
+        constexpr int LANES = HD / 4;
+        if (d4 < HD / 8) dot = dot8(load8(q_rot + h * HD + 8 * d4), load8(k_new + 8 * d4), 0.f);
+#pragma unroll
+        for (int x = LANES / 2; x >= 1; x /= 2) dot += __shfl_xor(dot, x);
+        dot *= 1.44269504088896341f / sqrtf((float)HD);
+        const float M = fmaxf(m, dot), f = __builtin_amdgcn_exp2f(m - M), w = __builtin_amdgcn_exp2f(dot - M), inv = 1.0f / (f * l + w);
+        half_t *row = out + (size_t)z * ldo + (size_t)(kvh * G + h) * HD + 4 * d4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) row[e] = (half_t)((f * o[e] + w * (float)v_new[e]) * inv);
+    }
+    // the new key and value into the caches
+    if (tid >= 64 * (AS_DIRECT_WAVES - 1)) {
+        if (lane < HD / 8) store8(kc + (size_t)(s.first + s.tail) * HD + lane * 8, load8(k_new + lane * 8));
+        for (int d = lane; d < HD; d += 64) vc[(size_t)d * max_pos + s.first + s.tail] = vn[d];
+    }
+}
+
+// Tiles (128 keys at head size 128, 256 at the others) up to which that is faster than two launches, one more at the smaller
+// head sizes.  Measured on 1, 4 and 16 sequences, direct against parts: head size 128, three tiles 9.3 / 9.3 / 9.5 against 10.8 /
+// 10.8 / 13.3 us, five 11.9 / 12.0 / 12.1 against 10.8 / 10.8 / 13.5; head size 64, five 10.2 / 10.3 / 10.4 against 10.7, nine 15.3
+// against 10.7; head size 32, five 7.9 / 8.1 / 8.1 against 10.7.
+#define AS_DIRECT_TILES 4
+// Workgroups per KV head: two on each of the 256 compute units.
 static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 * AS_PER_CU ? 256 * AS_PER_CU / n_kv_heads : 1; }
 
 template <int HD, int G, int QT, bool DEV> static int launch_shared(const SharedArgs &a, const AsPlan &pl, hipStream_t s) {
-    const size_t smem = sizeof(half_t) * as_lds_halves<HD>();
+    const size_t smem = as_lds_bytes<HD, QT, AS_WAVES>() > as_lds_bytes<HD, 1, AS_WAVES>() ? as_lds_bytes<HD, QT, AS_WAVES>() : as_lds_bytes<HD, 1, AS_WAVES>();
     auto kern = attn_shared_part_kernel<HD, G, QT, DEV>;
     static std::atomic<uint64_t> attr_done{0};
     if (smem > 48 * 1024) {
@@ -538,7 +637,22 @@ template <int HD, int G, int QT, bool DEV> static int launch_shared(const Shared
     return LLM_OK;
 }
 
+template <int HD, int G, bool DEV> static int launch_direct(const SharedArgs &a, hipStream_t s) {
+    const size_t smem = as_lds_bytes<HD, 1, AS_DIRECT_WAVES>();
+    auto kern = attn_shared_direct_kernel<HD, G, DEV>;
+    static std::atomic<uint64_t> attr_done{0};
+    if (smem > 48 * 1024) {
+        int rc = llm_ensure_max_smem((const void *)kern, smem, attr_done);
+        if (rc != LLM_OK) return rc;
+    }
+    kern<<<dim3(a.n_kv_heads, a.batch), dim3(64 * AS_DIRECT_WAVES), smem, s>>>(a.qkv, a.table, a.out, a.n_kv_heads, a.ldq, a.ldo, a.prefix_max, a.max_pos, a);
+    LLM_LAUNCH_CHECK("attn_shared_direct_kernel");
+    return LLM_OK;
+}
+
 template <int HD, int G> static int launch_shared(const SharedArgs &a, void *ws, hipStream_t s) {
+    constexpr int SK = AsShape<HD, 1, AS_DIRECT_WAVES>::SK;
+    if ((a.max_prefix + SK - 1) / SK + (a.max_tail + SK - 1) / SK <= (HD >= 128 ? AS_DIRECT_TILES : AS_DIRECT_TILES + 1)) return a.desc ? launch_direct<HD, G, true>(a, s) : launch_direct<HD, G, false>(a, s);
     const int rows = a.batch * G;
     AsPlan pl = {};
     pl.wgs = as_wgs(a.n_kv_heads);
