@@ -377,7 +377,7 @@ struct LpCut {
     int nl, chunk_len, chunks;
 };
 static LpCut lp_cut_row(int rows, int vocab) {
-    const int target = 256; // workgroups
+    const int target = 512; // workgroups
     int want = (target + rows - 1) / rows;
     if (want > LP_MAX_CHUNKS) want = LP_MAX_CHUNKS;
     int len = (vocab + want - 1) / want;
@@ -415,6 +415,7 @@ int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temp
     LLM_REQUIRE(((uintptr_t)logits & 1u) == 0 && aligned16(workspace) &&
                     (((uintptr_t)ids | (uintptr_t)logprob | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logprob) & 3u) == 0,
                 "llm_logprobs: logits must be aligned to 2 bytes, the workspace to 16, the others to 4");
+    if (rows == 0) return LLM_OK;
     LpArgs a = {};
     a.ld = (size_t)ld;
     a.vocab = vocab;

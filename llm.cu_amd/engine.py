@@ -184,6 +184,44 @@ class Engine:
         lib().llama3_decode_batch(engines[0].model.handle, caches, tok, B, out)
         return [int(x) for x in out]
 
+    def fork(self, engines):
+        """engines (1..16, same configuration) become copies of this one: cached rows, ids, position, last logits."""
+        lib().llama3_fork(self.cache, (capi.HOST_ABI["init_cache"][0] * len(engines))(*[e.cache for e in engines]), len(engines))
+
+    def set_shared_prefix(self, mode):
+        """Batched steps with this engine first read rows that all sequences share once: never (0), where faster (1), always (2)."""
+        lib().llama3_set_shared_prefix(self.cache, mode)
+
+    def shared_prefix_steps(self):
+        return lib().llama3_shared_prefix_steps(self.cache)
+
+    def _logprobs(self, fn, rows, ids, k, temperature):
+        ids = np.ascontiguousarray(ids, dtype=np.int32).reshape(rows, -1)
+        lp, ent = np.empty(ids.shape, np.float32), np.empty(rows, np.float32)
+        ti, tl = np.empty((rows, k), np.int32), np.empty((rows, k), np.float32)
+        fn(self.cache, temperature, ids.ctypes.data, ids.shape[1], lp.ctypes.data, ent.ctypes.data, k, ti.ctypes.data, tl.ctypes.data)
+        return lp, ent, ti, tl
+
+    def logprobs(self, ids=(), k=0, temperature=1.0):
+        """(log probabilities of ids, entropy, top ids, their log probabilities) of the last row processed."""
+        lp, ent, ti, tl = self._logprobs(lib().llama3_logprobs, 1, ids, k, temperature)
+        return lp[0], float(ent[0]), ti[0], tl[0]
+
+    def batch_logprobs(self, ids, k=0, temperature=1.0):
+        """The same for every sequence of the last decode_batch that began with this engine; ids [batch] or [batch, n]."""
+        return self._logprobs(lib().llama3_batch_logprobs, len(ids), ids, k, temperature)
+
+    def score(self, tokens, k=0, temperature=1.0):
+        """prefill that rates the text: (greedy next id, logprob [n] -- of tokens[i + 1] at i, NaN at the end --, entropy [n],
+        top ids [n, k], their log probabilities [n, k])."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        n = tokens.size
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        ti, tl = np.empty((n, k), np.int32), np.empty((n, k), np.float32)
+        nxt = lib().llama3_score(self.model.handle, self.cache, tokens.ctypes.data, n, temperature, lp.ctypes.data, ent.ctypes.data, k,
+                                 ti.ctypes.data, tl.ctypes.data)
+        return nxt, lp, ent, ti, tl
+
     def batch_logits(self, b):
         out = np.empty(self.cfg.vocab, np.uint16)
         lib().llama3_read_batch_logits(self.cache, b, out.ctypes.data)

@@ -13,6 +13,7 @@
 //   scores, softmax, P.V      -> llm_attn_prefill / llm_attn_decode over the cache
 //   copy + O projection, add  -> llm_linear with the residual in its epilogue
 //   gate/up+SiLU, down, add   -> llm_linear_swiglu, llm_linear with residual
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -96,6 +97,26 @@ struct Engine {
     int32_t *b_ids_host = nullptr;
     llm_graph_t b_graph[17][2] = {};
     bool b_ran[17][2] = {};
+    int b_rows = 0; // sequences of the last batched step (rows of b_logits)
+    // Rows that other caches hold bit for bit, from llama3_fork: caches with a mark of the same id agree on rows 0 .. len - 1.
+    // Marks grow in len; only llama3_cache_reset takes rows back, and with them the marks.
+    struct SharedRows {
+        uint64_t id;
+        int len;
+    };
+    std::vector<SharedRows> marks;
+    int shared_mode = 1;    // 0: batched steps never read a shared prefix once for all, 1: where it is faster, 2: always
+    long shared_steps = 0;  // batched steps with this cache as sequence 0 that did
+    llm_shared_desc *b_shared = nullptr, *b_shared_host = nullptr;
+    void *b_ws_shared = nullptr;
+    llm_graph_t b_shared_graph[17] = {};
+    bool b_shared_ran[17] = {};
+    // log probabilities (llama3_logprobs, llama3_batch_logprobs, llama3_score): device buffers for LP_ROWS rows, a pinned
+    // mirror of the results, the logits of a scored pass
+    int32_t *lp_ids = nullptr, *lp_top_ids = nullptr;
+    float *lp_out = nullptr, *lp_entropy = nullptr, *lp_top = nullptr;
+    void *lp_ws = nullptr;
+    llm_half *score_logits = nullptr;
     llm_event_t ev[4] = {nullptr, nullptr, nullptr, nullptr};
 };
 
@@ -105,6 +126,14 @@ const int LONG_ATTN_FROM = 512; // cached positions from which the span + merge 
 // wait for queries and angles, about 4 us per launch) costs more than the smaller RoPE launch saves (5 us at any size
 // up to a thousand rows).  Same bits either way.
 constexpr int ROPE_IN_ATTENTION_FROM = 4096;
+
+// Batched steps of forks read the shared prefix once for all from this many shared positions on, and where batch times
+// positions makes up for the second launch.  Measured, attention of a layer (8B heads), every cache for itself against shared:
+// 2 sequences, 1024 positions 10.3 against 11.8 us, 2048 12.8 against 12.1; 4 sequences, 512 10.7 against 11.9, 1024 12.8 against
+// 11.9; 8 sequences, 512 14.5 against 12.0; 16 sequences, 256 11.9 against 13.8, 512 21.7 against 14.2, 8192 108 against 21.5.
+constexpr int SHARED_FROM = 512, SHARED_FROM_ROWS = 4096;
+constexpr size_t MAX_MARKS = 8;
+constexpr int LP_ROWS = 512; // rows of logits that llama3_score holds at a time
 
 Engine *eng(const CudaCache *c) {
     if (!c || !c->engine) llama3_fail("CudaCache was not created by init_cache");
@@ -166,6 +195,10 @@ void drop_graph(Engine *e) {
             if (g) llm_graph_destroy(g);
             g = nullptr;
         }
+    for (llm_graph_t &g : e->b_shared_graph) {
+        if (g) llm_graph_destroy(g);
+        g = nullptr;
+    }
 }
 
 // The captured decode graphs hold the weight pointers of the model they were captured with.  A call
@@ -494,7 +527,9 @@ int step_one(Engine *e, const Llama3 *m, int token, llm_half *logits_host) {
 
 // One batched decode step on e0's stream from device state: ids in e0->b_ids, caches and positions in e0->b_desc;
 // leaves the greedy ids in e0->b_ids and the logits in e0->b_logits.  Nothing in it depends on host values that
-// change from step to step, so it can be captured.  form: 0 every position below LONG_ATTN_FROM, 1 otherwise.
+// change from step to step, so it can be captured.  form: 0 every position below LONG_ATTN_FROM, 1 otherwise, SHARED_FORM caches,
+// positions and the prefix that all share in e0->b_shared.
+constexpr int SHARED_FORM = 2;
 void issue_batch_step(Engine *e0, const Llama3 *m, int batch, int form) {
     const ModelConfig &c = e0->cfg;
     const int d = c.d_model, hd = c.head_dim, Hq = c.n_heads, Hkv = c.n_kv_heads, F = c.ffn_dim;
@@ -512,9 +547,15 @@ void issue_batch_step(Engine *e0, const Llama3 *m, int batch, int form) {
             llama3_check(llm_linear(e0->xn, d, w.wk, nullptr, 0, e0->qkv + qd, QKV, batch, kvd, d, s), "llm_linear(k)");
             llama3_check(llm_linear(e0->xn, d, w.wv, nullptr, 0, e0->qkv + qd + kvd, QKV, batch, kvd, d, s), "llm_linear(v)");
         }
-        llama3_check(llm_attn_decode_rope_batch_dev(e0->qkv, QKV, e0->b_desc, (size_t)l * e0->kv_layer_elems, batch, form, e0->attn,
+        if (form == SHARED_FORM)
+            llama3_check(llm_attn_decode_rope_shared_dev(e0->qkv, QKV, e0->b_shared, (size_t)l * e0->kv_layer_elems,
+                                                         (size_t)l * e0->kv_layer_elems, c.max_pos, c.max_pos, c.max_pos - 1, batch,
+                                                         e0->attn, qd, e0->rope_table, Hq, Hkv, hd, c.max_pos, e0->b_ws_shared, s),
+                         "llm_attn_decode_rope_shared_dev");
+        else
+            llama3_check(llm_attn_decode_rope_batch_dev(e0->qkv, QKV, e0->b_desc, (size_t)l * e0->kv_layer_elems, batch, form, e0->attn,
                                                     qd, e0->rope_table, Hq, Hkv, hd, c.max_pos, e0->b_ws_attn, s),
-                     "llm_attn_decode_rope_batch_dev");
+                         "llm_attn_decode_rope_batch_dev");
         llama3_check(llm_linear(e0->attn, qd, w.wo, e0->x, d, e0->x, d, batch, d, qd, s), "llm_linear(o)");
         llama3_check(llm_rmsnorm(e0->x, w.post_ln, e0->xn, batch, d, c.rms_eps, s), "llm_rmsnorm");
         llama3_check(llm_linear_swiglu(e0->xn, d, w.wg, w.wu, e0->ffn, F, batch, F, d, s), "llm_linear_swiglu");
@@ -525,6 +566,66 @@ void issue_batch_step(Engine *e0, const Llama3 *m, int batch, int form) {
                  "llm_linear(lm_head)");
     llama3_check(llm_argmax_f16_rows(e0->b_logits, c.vocab, batch, c.vocab, e0->b_ids, e0->b_ws_argmax, s),
                  "llm_argmax_f16_rows");
+}
+
+bool same_config(const ModelConfig &a, const ModelConfig &b) {
+    return a.max_pos == b.max_pos && a.d_model == b.d_model && a.n_layers == b.n_layers && a.vocab == b.vocab &&
+           a.n_heads == b.n_heads && a.n_kv_heads == b.n_kv_heads && a.head_dim == b.head_dim;
+}
+
+// Rows that all of the caches hold bit for bit.
+int rows_in_common(Engine *const *es, int n) {
+    for (size_t i = es[0]->marks.size(); i-- > 0;) { // longest first
+        const Engine::SharedRows &m = es[0]->marks[i];
+        bool all = true;
+        for (int b = 1; all && b < n; ++b) {
+            all = false;
+            for (const Engine::SharedRows &o : es[b]->marks) all = all || o.id == m.id;
+        }
+        if (all) return m.len;
+    }
+    return 0;
+}
+
+void prepare_logprobs(Engine *e) {
+    if (e->lp_ws) return;
+    size_t ws = 0;
+    for (int rows = 1; rows <= LP_ROWS; ++rows) {
+        const size_t need = llm_logprobs_workspace_bytes(rows, e->cfg.vocab, LLM_LOGPROBS_MAX_TOP);
+        ws = need > ws ? need : ws;
+    }
+    ws = (ws + 3) / 4 * 4;
+    e->lp_ids = dmalloc<int32_t>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_IDS, "llm_malloc(given tokens)");
+    e->lp_out = dmalloc<float>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_IDS, "llm_malloc(log probabilities)");
+    e->lp_entropy = dmalloc<float>(LP_ROWS, "llm_malloc(entropies)");
+    e->lp_top_ids = dmalloc<int32_t>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_TOP, "llm_malloc(alternatives)");
+    e->lp_top = dmalloc<float>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_TOP, "llm_malloc(alternatives' log probabilities)");
+    e->lp_ws = dmalloc<char>(ws, "llm_malloc(log probability workspace)");
+    llama3_check(llm_fill_zero(e->lp_ws, ws, e->stream), "zero log probability workspace");
+}
+
+void check_logprob_args(const Engine *e, int n_ids, int k, const void *ids, const void *logprob, const void *top_ids, const void *top) {
+    if (n_ids < 0 || n_ids > LLM_LOGPROBS_MAX_IDS) llama3_fail("log probabilities of %d given tokens (0..%d)", n_ids, LLM_LOGPROBS_MAX_IDS);
+    if (k < 0 || k > LLM_LOGPROBS_MAX_TOP || k > e->cfg.vocab) llama3_fail("top %d alternatives (0..%d, at most the vocabulary)", k, LLM_LOGPROBS_MAX_TOP);
+    if ((n_ids > 0 && (!ids || !logprob)) || (k > 0 && (!top_ids || !top))) llama3_fail("log probabilities: null pointer");
+}
+
+// llm_logprobs on up to LP_ROWS rows of device logits, host ids in, host results out (any of them null: not wanted).
+void logprob_rows(Engine *e, const llm_half *logits, int rows, float temperature, const int *ids, int n_ids, float *logprob,
+                  float *entropy, int k, int *top_ids, float *top) {
+    prepare_logprobs(e);
+    llm_stream_t s = e->stream;
+    if (n_ids > 0) llama3_check(llm_memcpy_h2d(e->lp_ids, ids, sizeof(int) * (size_t)rows * n_ids, s), "H2D given tokens");
+    llama3_check(llm_logprobs(logits, e->cfg.vocab, rows, e->cfg.vocab, temperature, e->lp_ids, n_ids, e->lp_out, e->lp_entropy, k,
+                              e->lp_top_ids, e->lp_top, e->lp_ws, s),
+                 "llm_logprobs");
+    if (n_ids > 0) llama3_check(llm_memcpy_d2h(logprob, e->lp_out, sizeof(float) * (size_t)rows * n_ids, s), "D2H log probabilities");
+    if (entropy) llama3_check(llm_memcpy_d2h(entropy, e->lp_entropy, sizeof(float) * (size_t)rows, s), "D2H entropies");
+    if (k > 0) {
+        llama3_check(llm_memcpy_d2h(top_ids, e->lp_top_ids, sizeof(int) * (size_t)rows * k, s), "D2H alternatives");
+        llama3_check(llm_memcpy_d2h(top, e->lp_top, sizeof(float) * (size_t)rows * k, s), "D2H alternatives");
+    }
+    llama3_check(llm_stream_sync(s), "stream sync");
 }
 
 } // namespace
@@ -624,12 +725,14 @@ extern "C" void free_cache(CudaCache *C) {
         drop_graph(e);
         void *bufs[] = {e->x, e->xn, e->qkv, e->attn, e->ffn, e->logits, e->kc, e->vc, e->rope_table,
                         e->d_tokens, e->d_pos, e->d_token, e->ao_ring, e->ws_attn, e->ws_lm, e->trace_dev, e->inject_dev,
-                        e->b_logits, e->b_ids, e->b_ws_attn, e->b_ws_argmax, e->b_desc};
+                        e->b_logits, e->b_ids, e->b_ws_attn, e->b_ws_argmax, e->b_desc, e->b_shared, e->b_ws_shared, e->lp_ids,
+                        e->lp_top_ids, e->lp_out, e->lp_entropy, e->lp_top, e->lp_ws, e->score_logits};
         for (void *b : bufs) llm_free(b);
         for (auto ev : e->ev) llm_event_destroy(ev);
         llm_stream_destroy(e->stream);
         llm_free_host(e->h_stage);
         if (e->b_desc_host) llm_free_host(e->b_desc_host);
+        if (e->b_shared_host) llm_free_host(e->b_shared_host);
         if (e->b_ids_host) llm_free_host(e->b_ids_host);
         if (e->h_select) llm_free_host(e->h_select);
         if (e->d_select) llm_free(e->d_select);
@@ -663,6 +766,7 @@ extern "C" void llama3_cache_reset(CudaCache *C) {
     Engine *e = eng(C);
     e->pos = 0;
     e->tokens.clear();
+    e->marks.clear();
     e->dev_pos_valid = false;
     e->dev_next = -1;
 }
@@ -744,7 +848,7 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
     Engine *e0 = eng(caches[0]);
     const ModelConfig &c = e0->cfg;
     bind_model(e0, m);
-    const int d = c.d_model, hd = c.head_dim, Hq = c.n_heads;
+    const int hd = c.head_dim, Hq = c.n_heads;
     llm_stream_t s = e0->stream;
     Engine *es[16];
     int pos[16];
@@ -752,9 +856,7 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
         es[b] = eng(caches[b]);
         for (int a = 0; a < b; ++a)
             if (es[a] == es[b]) llama3_fail("llama3_decode_batch: sequence %d and %d share a cache", a, b);
-        const ModelConfig &cb = es[b]->cfg;
-        if (cb.max_pos != c.max_pos || cb.d_model != d || cb.n_layers != c.n_layers || cb.vocab != c.vocab ||
-            cb.n_kv_heads != c.n_kv_heads || cb.head_dim != c.head_dim)
+        if (!same_config(es[b]->cfg, c))
             llama3_fail("llama3_decode_batch: cache %d has a different configuration", b);
         if (es[b]->pos + 1 > c.max_pos) llama3_fail("sequence of %d tokens exceeds max_pos %d", es[b]->pos + 1, c.max_pos);
         if (tokens[b] < 0 || tokens[b] >= c.vocab) llama3_fail("token id %d outside the vocabulary", tokens[b]);
@@ -794,9 +896,31 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
     }
     llama3_check(llm_memcpy_h2d(e0->b_ids, e0->b_ids_host, sizeof(int32_t) * (size_t)batch, s), "H2D ids");
     llama3_check(llm_memcpy_h2d(e0->b_desc, e0->b_desc_host, sizeof(llm_batch_desc), s), "H2D batch descriptor");
-    const int form = long_form ? 1 : 0;
-    if (e0->use_graph && e0->b_ran[batch][form]) {
-        llm_graph_t &g = e0->b_graph[batch][form];
+    int form = long_form ? 1 : 0;
+    const int prefix = e0->shared_mode ? rows_in_common(es, batch) : 0;
+    if (prefix > 0 && (e0->shared_mode == 2 || (batch > 1 && prefix >= SHARED_FROM && batch * prefix >= SHARED_FROM_ROWS))) {
+        form = SHARED_FORM;
+        if (!e0->b_shared) {
+            const size_t wsb = (llm_attn_shared_workspace_bytes(Hq, c.n_kv_heads, hd, 16) + 3) / 4 * 4;
+            e0->b_ws_shared = dmalloc<char>(wsb, "llm_malloc(shared attention workspace)");
+            llama3_check(llm_fill_zero(e0->b_ws_shared, wsb, s), "zero workspace");
+            void *hp = nullptr;
+            llama3_check(llm_malloc_host(&hp, sizeof(llm_shared_desc)), "llm_malloc_host(shared batch descriptor)");
+            e0->b_shared_host = (llm_shared_desc *)hp;
+            e0->b_shared = dmalloc<llm_shared_desc>(1, "llm_malloc(shared batch descriptor)");
+        }
+        // the prefix is read from sequence 0's own rows: every cache holds them
+        e0->b_shared_host->k_prefix = e0->kc;
+        e0->b_shared_host->v_prefix = e0->vc;
+        e0->b_shared_host->prefix_len = prefix;
+        e0->b_shared_host->row0 = 0;
+        e0->b_shared_host->seq = *e0->b_desc_host;
+        llama3_check(llm_memcpy_h2d(e0->b_shared, e0->b_shared_host, sizeof(llm_shared_desc), s), "H2D shared batch descriptor");
+        ++e0->shared_steps;
+    }
+    bool &ran = form == SHARED_FORM ? e0->b_shared_ran[batch] : e0->b_ran[batch][form];
+    if (e0->use_graph && ran) {
+        llm_graph_t &g = form == SHARED_FORM ? e0->b_shared_graph[batch] : e0->b_graph[batch][form];
         if (!g) {
             llama3_check(llm_graph_capture_begin(s), "graph capture begin");
             issue_batch_step(e0, m, batch, form);
@@ -805,8 +929,9 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
         llama3_check(llm_graph_launch(g, s), "graph launch");
     } else {
         issue_batch_step(e0, m, batch, form);
-        e0->b_ran[batch][form] = true;
+        ran = true;
     }
+    e0->b_rows = batch;
     llama3_check(llm_memcpy_d2h(e0->b_ids_host, e0->b_ids, sizeof(int32_t) * (size_t)batch, s), "D2H tokens");
     llama3_check(llm_stream_sync(s), "stream sync");
     for (int b = 0; b < batch; ++b) {
@@ -815,6 +940,97 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
         es[b]->pos += 1;
         es[b]->dev_pos_valid = false; // the batched step keeps no per-cache position on the device
     }
+}
+
+// ---------------------------------------------------------------------------
+// Several answers to one prompt: the rows of a cache copied into others (every copy stands for itself afterwards; what they have
+// in common is remembered, and batched steps read it once), log probabilities of what is in device memory anyway.
+// ---------------------------------------------------------------------------
+extern "C" void llama3_fork(CudaCache *src, CudaCache *const *dsts, int n) {
+    Engine *e = eng(src);
+    const ModelConfig &c = e->cfg;
+    if (n < 1 || n > 16 || !dsts) llama3_fail("llama3_fork: %d destinations (1..16)", n);
+    Engine *es[16];
+    int from = e->pos; // rows in front of it are in every destination already
+    for (int i = 0; i < n; ++i) {
+        es[i] = eng(dsts[i]);
+        if (es[i] == e) llama3_fail("llama3_fork: destination %d is the source", i);
+        for (int j = 0; j < i; ++j)
+            if (es[j] == es[i]) llama3_fail("llama3_fork: destinations %d and %d share a cache", j, i);
+        if (!same_config(es[i]->cfg, c)) llama3_fail("llama3_fork: cache %d has a different configuration", i);
+        Engine *pair[2] = {e, es[i]};
+        const int same = rows_in_common(pair, 2);
+        from = same < from ? same : from;
+        llama3_check(llm_stream_sync(es[i]->stream), "stream sync"); // its own work has finished
+    }
+    llm_stream_t s = e->stream;
+    llm_half *ks[16], *vs[16];
+    for (int i = 0; i < n; ++i) {
+        ks[i] = es[i]->kc;
+        vs[i] = es[i]->vc;
+        llama3_check(llm_memcpy_d2d(es[i]->logits, e->logits, sizeof(llm_half) * (size_t)c.vocab, s), "D2D logits");
+    }
+    llama3_check(llm_kv_fork(e->kc, e->vc, c.max_pos, from, ks, vs, n, c.max_pos, from, e->pos - from, c.n_layers, c.n_kv_heads,
+                             c.head_dim, s),
+                 "llm_kv_fork");
+    if (e->pos > 0 && (e->marks.empty() || e->marks.back().len < e->pos)) {
+        static std::atomic<uint64_t> next_id{1};
+        if (e->marks.size() == MAX_MARKS) e->marks.erase(e->marks.begin() + 1); // the first one, the prompt's, stays
+        e->marks.push_back({next_id.fetch_add(1), e->pos});
+    }
+    for (int i = 0; i < n; ++i) {
+        es[i]->tokens = e->tokens;
+        es[i]->pos = e->pos;
+        es[i]->marks = e->marks;
+        es[i]->dev_pos_valid = false; // its device copies of position and ids are those of what it held before
+        es[i]->dev_next = -1;
+    }
+    llama3_check(llm_stream_sync(s), "stream sync");
+}
+
+extern "C" void llama3_set_shared_prefix(CudaCache *C, int mode) {
+    if (mode < 0 || mode > 2) llama3_fail("llama3_set_shared_prefix: mode %d (0..2)", mode);
+    eng(C)->shared_mode = mode;
+}
+
+extern "C" long llama3_shared_prefix_steps(const CudaCache *C) { return eng(C)->shared_steps; }
+
+extern "C" void llama3_logprobs(CudaCache *C, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
+                                int *top_ids, float *top_logprob) {
+    Engine *e = eng(C);
+    check_logprob_args(e, n_ids, k, ids, logprob, top_ids, top_logprob);
+    if (e->pos == 0) llama3_fail("llama3_logprobs: no row has been processed");
+    logprob_rows(e, e->logits, 1, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
+}
+
+extern "C" void llama3_batch_logprobs(CudaCache *C0, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
+                                      int *top_ids, float *top_logprob) {
+    Engine *e = eng(C0);
+    check_logprob_args(e, n_ids, k, ids, logprob, top_ids, top_logprob);
+    if (e->b_rows == 0) llama3_fail("llama3_batch_logprobs: no batch step has run");
+    logprob_rows(e, e->b_logits, e->b_rows, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
+}
+
+extern "C" int llama3_score(Llama3 *m, CudaCache *C, const int *tokens, int n, float temperature, float *logprob, float *entropy, int k,
+                            int *top_ids, float *top_logprob) {
+    Engine *e = eng(C);
+    const ModelConfig &c = e->cfg;
+    check_logprob_args(e, 1, k, tokens, logprob, top_ids, top_logprob);
+    const int next = run_pass(e, m, tokens, n); // leaves the residual stream of its rows in e->x
+    llm_stream_t s = e->stream;
+    const int d = c.d_model, at_once = n < LP_ROWS ? n : LP_ROWS;
+    if (!e->score_logits) e->score_logits = dmalloc<llm_half>((size_t)(c.max_pos < LP_ROWS ? c.max_pos : LP_ROWS) * c.vocab, "llm_malloc(logits of a scored pass)");
+    llama3_check(llm_rmsnorm(e->x, m->norm->d_fp16_tensor, e->xn, n, d, c.rms_eps, s), "llm_rmsnorm");
+    std::vector<int> given((size_t)n);
+    for (int i = 0; i < n; ++i) given[i] = i + 1 < n ? tokens[i + 1] : -1; // no token is known behind the last one
+    for (int r0 = 0; r0 < n; r0 += at_once) {
+        const int rows = n - r0 < at_once ? n - r0 : at_once;
+        llama3_check(llm_linear(e->xn + (size_t)r0 * d, d, m->lm_head->d_fp16_tensor, nullptr, 0, e->score_logits, c.vocab, rows, c.vocab, d, s),
+                     "llm_linear(lm_head)");
+        logprob_rows(e, e->score_logits, rows, temperature, given.data() + r0, 1, logprob + r0, entropy ? entropy + r0 : nullptr, k,
+                     top_ids ? top_ids + (size_t)r0 * k : nullptr, top_logprob ? top_logprob + (size_t)r0 * k : nullptr);
+    }
+    return next;
 }
 
 // fp16 logits of sequence b after the last llama3_decode_batch() in which caches[0] was this cache

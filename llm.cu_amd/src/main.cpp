@@ -4,10 +4,13 @@
 //
 //   llama3_main [--config tiny|8b] [--seed S] [--weights a.safetensors[,b,...]]
 //               [--prompt-len N] [--decode N] [--max-pos N] [--no-graph]
-//               [--tokenizer tokenizer.json --text "question" [--sample]]
+//               [--tokenizer tokenizer.json --text "question" [--sample]] [--answers N]
 // With --tokenizer and --text the reference's chat turn runs instead (main.cu:98-130): chat template,
 // tokenize, inference() per token until a special id (>= 128000) or the context limit, decoded text
 // printed as it comes; --sample uses the reference's sampler instead of the argmax.
+// With --answers N (2..16) the prompt runs once, its cache is forked into N sequences that are sampled side by side (the
+// reference's sampler settings), and the answers are listed by the mean log probability of their tokens.
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -17,11 +20,51 @@
 #include "llama3_host.h"
 #include "llmcu_hip.h"
 
+// N sampled answers of n_tokens each to one prompt, the likeliest first.
+static void sampled_answers(Llama3 *model, CudaCache *prompt_cache, const ModelConfig &cfg, const std::vector<int> &prompt, int n, int n_tokens,
+                            int graph) {
+    const float temperature = 0.7f, top_p = 0.9f; // inference.cu:27-29
+    const int top_k = 50;
+    std::vector<CudaCache *> caches;
+    for (int i = 0; i < n; ++i) {
+        caches.push_back(init_cache_cfg(model, &cfg));
+        llama3_set_use_graph(caches[i], graph);
+    }
+    llama3_prefill(model, prompt_cache, prompt.data(), (int)prompt.size());
+    llama3_fork(prompt_cache, caches.data(), n);
+    std::vector<llm_half> logits(cfg.vocab);
+    std::vector<float> scratch(cfg.vocab), sum(n, 0.f), lp(n);
+    std::vector<std::vector<int>> answers(n);
+    std::vector<int> ids(n), greedy(n);
+    for (int step = 0; step < n_tokens; ++step) {
+        for (int i = 0; i < n; ++i) {
+            if (step == 0) llama3_read_logits(caches[i], logits.data());
+            else llama3_read_batch_logits(caches[0], i, logits.data());
+            ids[i] = llama3_sample_with(cfg.vocab, temperature, top_k, top_p, scratch.data(), logits.data());
+            answers[i].push_back(ids[i]);
+            if (step == 0) llama3_logprobs(caches[i], temperature, &ids[i], 1, &lp[i], nullptr, 0, nullptr, nullptr);
+        }
+        if (step > 0) llama3_batch_logprobs(caches[0], temperature, ids.data(), 1, lp.data(), nullptr, 0, nullptr, nullptr);
+        for (int i = 0; i < n; ++i) sum[i] += lp[i];
+        if (step + 1 < n_tokens) llama3_decode_batch(model, caches.data(), ids.data(), n, greedy.data());
+    }
+    std::vector<int> order(n);
+    for (int i = 0; i < n; ++i) order[i] = i;
+    std::sort(order.begin(), order.end(), [&](int a, int b) { return sum[a] != sum[b] ? sum[a] > sum[b] : a < b; });
+    for (int i : order) {
+        printf("answer %d, mean log probability %.4f:", i, sum[i] / n_tokens);
+        for (int t : answers[i]) printf(" %d", t);
+        printf("\n");
+    }
+    printf("batched steps that read the prompt's rows once: %ld of %d\n", llama3_shared_prefix_steps(caches[0]), n_tokens - 1);
+    for (CudaCache *c : caches) free_cache(c);
+}
+
 int main(int argc, char **argv) {
     std::string config = "tiny", weights, tokenizer_path, text;
     bool sample = false;
     uint64_t seed = 1234;
-    int prompt_len = 16, decode = 32, max_pos = 0, graph = 1;
+    int prompt_len = 16, decode = 32, max_pos = 0, graph = 1, answers = 0;
     for (int i = 1; i < argc; ++i) {
         std::string a = argv[i];
         auto next = [&]() -> const char * {
@@ -41,10 +84,15 @@ int main(int argc, char **argv) {
         else if (a == "--tokenizer") tokenizer_path = next();
         else if (a == "--text") text = next();
         else if (a == "--sample") sample = true;
+        else if (a == "--answers") answers = atoi(next());
         else {
             printf("Error: unknown option %s\n", a.c_str());
             return 1;
         }
+    }
+    if (answers != 0 && (answers < 2 || answers > 16 || decode < 1 || prompt_len < 1 || !tokenizer_path.empty())) {
+        printf("Error: --answers takes 2 to 16, with a prompt and a number of tokens and without --tokenizer\n");
+        return 1;
     }
     ModelConfig cfg = config == "8b" ? llama3_config_8b() : llama3_config_tiny();
     if (max_pos > 0) cfg.max_pos = max_pos;
@@ -114,6 +162,12 @@ int main(int argc, char **argv) {
 
     std::vector<int> prompt(prompt_len), out(decode);
     seeded_tokens(seed, prompt_len, cfg.vocab, prompt.data());
+    if (answers > 0) {
+        sampled_answers(model, cache, cfg, prompt, answers, decode, graph);
+        free_cache(cache);
+        free_llama3(model);
+        return 0;
+    }
     GenStats st;
     llama3_generate(model, cache, prompt.data(), prompt_len, decode, out.data(), &st);
     printf("tokens:");
