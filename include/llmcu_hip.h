@@ -278,7 +278,7 @@ int llm_attn_decode_rope_batch_dev(const uint16_t *qkv_dev, int ldq, const llm_b
  * Row r of every own cache ([n_kv_heads][max_pos][head_dim]) holds position row0 + r, 0 <= row0 <= prefix_len: 0 for caches
  * that hold the prefix too (their rows below prefix_len are not read), prefix_len for caches that hold the answers only.
  * positions[z] < row0 + max_pos; table_dev covers row0 + max_pos positions.  The prefix cache may be one of the own caches
- * (with row0 = 0); own caches are distinct.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
+ * (with row0 = 0 and prefix_max_pos = max_pos); own caches are distinct.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
  * 2 GiB.  Rows that hold no position yet may hold anything, NaN included.
  * Arithmetic: queries and the new key are rounded to fp16 after the rotation (llm_rope's results), products on the matrix
  * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32.  The order of the sums depends on the
@@ -294,7 +294,7 @@ int llm_attn_decode_rope_shared(const uint16_t *qkv_dev, int ldq, const uint16_t
 /* The same with caches, lengths and positions read from an llm_shared_desc in device memory when the kernels run (for
  * captured steps).  prefix_offset and cache_offset are added, in elements, to the prefix and own cache pointers.  The launch
  * is sized for prefixes of up to max_prefix positions and sequences with up to max_tail rows behind it: a descriptor's
- * longer prefix or tail, and positions outside the caches, are clamped to what is served. */
+ * longer prefix or tail, and positions outside the caches, are clamped to what is served (positions below row0 + max_pos). */
 typedef struct {
     const uint16_t *k_prefix, *v_prefix;
     int32_t prefix_len, row0;

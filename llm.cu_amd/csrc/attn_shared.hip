@@ -41,11 +41,11 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
     s.vp = reinterpret_cast<const half_t *>(d.v_prefix) + a.prefix_offset;
     s.kc = reinterpret_cast<half_t *>(d.seq.k_cache[z]) + a.cache_offset;
     s.vc = reinterpret_cast<half_t *>(d.seq.v_cache[z]) + a.cache_offset;
-    int prefix = d.prefix_len, row0 = d.row0, tail = d.seq.pos[z] - d.prefix_len;
+    int prefix = d.prefix_len, row0 = d.row0, tail = (int)((uint32_t)d.seq.pos[z] - (uint32_t)d.prefix_len);
     if (DEV) {
         prefix = prefix < 0 ? 0 : prefix > a.max_prefix ? a.max_prefix : prefix;
         row0 = row0 < 0 ? 0 : row0 > prefix ? prefix : row0;
-        if (prefix - row0 > a.max_pos - 1) row0 = prefix - (a.max_pos - 1);
+        if (prefix - row0 > a.max_pos - 1) prefix = row0 + a.max_pos - 1; // positions stay below row0 + max_pos, as the table does
         const int most = a.max_tail < a.max_pos - 1 - (prefix - row0) ? a.max_tail : a.max_pos - 1 - (prefix - row0);
         tail = tail < 0 ? 0 : tail > most ? most : tail;
     }
@@ -740,6 +740,10 @@ int llm_attn_decode_rope_shared(const uint16_t *qkv, int ldq, const uint16_t *k_
         LLM_REQUIRE(k_caches[z] && v_caches[z] && aligned16(k_caches[z]) && aligned16(v_caches[z]), "%s: cache %d", name, z);
         LLM_REQUIRE(positions[z] >= prefix_len && (long long)positions[z] - row0 < max_pos, "%s: position %d (the prefix has %d, the caches hold %d..%lld)",
                     name, positions[z], prefix_len, row0, (long long)row0 + max_pos - 1);
+        // a prefix inside one of the own caches stays where it is only if row r of that cache is position r
+        LLM_REQUIRE(prefix_len == 0 || (k_caches[z] != k_prefix && v_caches[z] != v_prefix) ||
+                        (k_caches[z] == k_prefix && v_caches[z] == v_prefix && row0 == 0 && prefix_max_pos == max_pos),
+                    "%s: the prefix lies in cache %d, whose row 0 is not position 0 or whose size is another", name, z);
         for (int y = 0; y < z; ++y)
             LLM_REQUIRE(k_caches[y] != k_caches[z] && v_caches[y] != v_caches[z], "%s: sequences %d and %d share a cache", name, y, z);
         a.host.seq.k_cache[z] = k_caches[z];

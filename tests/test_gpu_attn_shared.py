@@ -120,6 +120,57 @@ def test_batches(gpu, B, heads):
     verify(run(gpu, c), expected(c))
 
 
+# The kernels have a one-launch form for short lengths and a two-launch form for long ones; a descriptor call is sized by its
+# bounds, so that generous ones take the long form at any length.
+def run_long(gpu, c):
+    return gpu.ops.attn_decode_rope_shared(c["qkv"], c["kp"], c["vp"], c["prefix"], c["kcs"], c["vcs"], c["positions"], c["row0"],
+                                           *c["heads"], dev=True, max_prefix=c["kp"].shape[1], max_tail=c["kcs"].shape[2] - 1)
+
+
+@pytest.mark.parametrize("heads", SHAPES)
+@pytest.mark.parametrize("tails_only", [False, True])
+def test_every_head_shape_at_length(gpu, heads, tails_only):
+    c = case(21, 4, 1400, [0, 17, 70, 129], heads, tails_only)
+    say("shared attention, long", heads, "tails only" if tails_only else "full caches")
+    verify(run(gpu, c), expected(c))
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 7, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (8, 2, 32)])
+def test_short_lengths_in_the_long_form(gpu, prefix, heads):
+    c = case(22, 3, prefix, [0, 5, 66], heads, True, prefix_slack=8192)
+    say("long form, prefix", prefix, heads)
+    verify(run_long(gpu, c), expected(c))
+
+
+@pytest.mark.parametrize("prefix", [959, 960, 961, 1023, 1024, 1025, 1087, 2049])
+@pytest.mark.parametrize("tails", [[0, 0], [1, 64], [63, 65], [200, 3]])
+def test_long_prefix_edges(gpu, prefix, tails):
+    c = case(23, 2, prefix, tails, (8, 2, 128), prefix % 2 == 0)
+    say("prefix", prefix, "tails", tails)
+    verify(run(gpu, c), expected(c))
+
+
+@pytest.mark.parametrize("B", [1, 2, 4, 7, 8, 9, 16])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (16, 2, 128), (8, 2, 32), (2, 2, 64)])
+def test_batches_at_length(gpu, B, heads):
+    """One, two and four query tiles, batches that do not fill them."""
+    c = case(24, B, 2100, [(11 * z) % 90 for z in range(B)], heads, True)
+    say("batch, long", B, heads)
+    verify(run(gpu, c), expected(c))
+
+
+def test_tails_longer_than_the_prefix(gpu):
+    c = case(25, 6, 65, [2000, 1, 700, 0, 1300, 64], (8, 2, 128), True)
+    verify(run(gpu, c), expected(c))
+
+
+def test_many_kv_heads(gpu):
+    """More KV heads than one workgroup each fills the chip with."""
+    c = case(26, 2, 300, [5, 40], (600, 600, 32), True, prefix_slack=8192)
+    verify(run_long(gpu, c), expected(c))
+
+
 def test_no_position_but_the_new_one(gpu):
     """Nothing cached at all: the output is the new value row."""
     c = case(5, 4, 0, [0, 0, 0, 0], (8, 2, 128), True)
@@ -186,6 +237,14 @@ def test_descriptor_beyond_its_bounds_is_clamped(gpu):
     assert all(np.array_equal(x, y) for x, y in zip(got, want))
     got = run(gpu, dict(c, positions=[-5, 2 ** 31 - 1]), dev=True, max_tail=20)
     want = run(gpu, dict(c, positions=[128, 128 + 20]), dev=True, max_tail=20)
+    assert all(np.array_equal(x, y) for x, y in zip(got, want))
+
+
+def test_descriptor_with_a_prefix_beyond_the_own_caches_is_clamped(gpu):
+    """Row 0 is position 0 and the prefix is longer than the caches: positions stay inside caches and (cos, sin) table."""
+    c = dict(case(27, 2, 128, [0, 0], (8, 2, 128), True), row0=0)
+    got = run(gpu, c, dev=True, max_prefix=128, max_tail=0)
+    want = run(gpu, dict(c, prefix=63, positions=[63, 63]), dev=True, max_prefix=128, max_tail=0)
     assert all(np.array_equal(x, y) for x, y in zip(got, want))
 
 

@@ -44,6 +44,8 @@ def shared(pkg, **over):
     (dict(qkv=A + 2), "aligned"), (dict(table=A + 8), "aligned"), (dict(ws=A + 4), "aligned"), (dict(kp=A + 8), "aligned"),
     (dict(ks=(A, A + 2)), "cache 1"), (dict(vs=(A + 8, A)), "cache 0"),
     (dict(ks=(A, A)), "share"), (dict(vs=(A, A)), "share"),
+    (dict(ks=(A + BIG, A), vs=(A + 2 * BIG, A), row0=100, pmax=256), "the prefix lies in cache 0"), (dict(ks=(A, A + BIG)), "the prefix lies in cache 1"),
+    (dict(ks=(A + BIG, A), vs=(A + 2 * BIG, A)), "whose size is another"),
 ])
 def test_shared_attention(pkg, over, text):
     refused(pkg, shared(pkg, **over), text)
