@@ -81,13 +81,15 @@ __device__ __forceinline__ LpStats lp_rebase(LpStats p, float M, float c) {
     return {M, f * p.s, f == 0.f ? 0.f : f * (p.t + d * p.s)};
 }
 
-// k-th largest of the lanes' keys (0: fewer than k lanes have one)
+// k-th largest of the lanes' keys (0: fewer than k lanes have one); two bits at a time, the three counts of a step side by side
 __device__ __forceinline__ uint32_t lp_kth_key(uint32_t key, int k) {
     uint32_t t = 0;
 #pragma unroll
-    for (int bit = 15; bit >= 0; --bit) {
-        const uint32_t trial = t | 1u << bit;
-        if (__popcll(__builtin_amdgcn_ballot_w64(key >= trial)) >= k) t = trial;
+    for (int bit = 14; bit >= 0; bit -= 2) {
+        const int c1 = __popcll(__builtin_amdgcn_ballot_w64(key >= (t | 1u << bit)));
+        const int c2 = __popcll(__builtin_amdgcn_ballot_w64(key >= (t | 2u << bit)));
+        const int c3 = __popcll(__builtin_amdgcn_ballot_w64(key >= (t | 3u << bit)));
+        t |= (c3 >= k ? 3u : c2 >= k ? 2u : c1 >= k ? 1u : 0u) << bit;
     }
     return t;
 }
@@ -105,18 +107,17 @@ __device__ __forceinline__ int lp_append(lp_word *list, int n, unsigned long lon
     return n + __popcll(who);
 }
 
-// How many of list[0 .. n8) are above a and above b: n8 is a multiple of eight (zeros fill the list up), eight words in flight.
-__device__ __forceinline__ void lp_ranks(const lp_word *list, int n8, lp_word a, lp_word b, int &ra, int &rb) {
+// How many of list[0 .. n8) are above w: n8 is a multiple of eight (zeros fill the list up), eight words in flight.
+__device__ __forceinline__ int lp_rank(const lp_word *list, int n8, lp_word w) {
+    int rank = 0;
     for (int j = 0; j < n8; j += 8) {
-        lp_pair w[4];
+        lp_pair x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const lp_pair *>(list + j + 2 * i);
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const lp_pair *>(list + j + 2 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ra += (w[i][0] > a) + (w[i][1] > a);
-            rb += (w[i][0] > b) + (w[i][1] > b);
-        }
+        for (int i = 0; i < 4; ++i) rank += (x[i][0] > w) + (x[i][1] > w);
     }
+    return rank;
 }
 
 // The k largest of a wavefront's n <= LP_LIST distinct words to the front of its list, largest first, zeros behind them
@@ -148,9 +149,9 @@ __device__ __forceinline__ void lp_cut(lp_word *list, int n, int k) {
     if (n <= 128) {
         if (lane < 8) list[n + lane] = 0ull;
         lp_wave_sync();
+        const int n8 = (n + 7) & ~7;
         const lp_word a = lane < n ? list[lane] : 0ull, b = lane + 64 < n ? list[lane + 64] : 0ull;
-        int ra = 0, rb = 0;
-        lp_ranks(list, (n + 7) & ~7, a, b, ra, rb);
+        const int ra = lp_rank(list, n8, a), rb = n > 64 ? lp_rank(list, n8, b) : 0;
         lp_wave_sync();
         if (a && ra < k) list[ra] = a;
         if (b && rb < k) list[rb] = b;
@@ -182,9 +183,9 @@ __device__ __forceinline__ void lp_join_waves(const lp_word *lists, int k, lp_wo
     __syncthreads();
     if (tid < LP_WAVES * k) {
         const lp_word mine = lists[tid / k * LP_LIST + tid % k];
-        int rank = 0, none = 0;
+        int rank = 0;
 #pragma unroll
-        for (int w = 0; w < LP_WAVES; ++w) lp_ranks(lists + w * LP_LIST, (k + 7) & ~7, mine, ~0ull, rank, none);
+        for (int w = 0; w < LP_WAVES; ++w) rank += lp_rank(lists + w * LP_LIST, (k + 7) & ~7, mine);
         if (mine && rank < k) best[rank] = mine;
     }
     __syncthreads();
@@ -342,11 +343,16 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         const LpStats p = lp_rebase({mine[0], mine[1], mine[2]}, M, c);
         st = {M, wave_sum(p.s), wave_sum(p.t)};
         if (k > 0) {
+            lp_word top = 0ull;
+#pragma unroll
+            for (int j = 0; j < LP_JOIN; ++j) top = w[j] > top ? w[j] : top;
+            const uint32_t kth = lp_kth_key(lp_word_key(top), k); // the same bound, on what the chunks listed
             n = 0;
 #pragma unroll
             for (int j = 0; j < LP_JOIN; ++j) {
-                const unsigned long long who = __builtin_amdgcn_ballot_w64(w[j] != 0ull);
-                if (who) n = lp_append(list, n, who, w[j] != 0ull, w[j]);
+                const bool mine_too = w[j] != 0ull && lp_word_key(w[j]) >= kth;
+                const unsigned long long who = __builtin_amdgcn_ballot_w64(mine_too);
+                if (who) n = lp_append(list, n, who, mine_too, w[j]);
             }
             lp_cut(list, n, k);
             __syncthreads();
