@@ -5,6 +5,15 @@
 //
 // Positions 0..prefix_len-1 come from one prefix cache, positions prefix_len..p_z-1 from the sequence's own cache (row r
 // holds position row0 + r), position p_z is the new token, whose rotated key and value are appended to the own cache.
+//
+// What bounds it: the bytes of the caches.  Per KV head and prefix position 2 hd halves are read for 4 hd batch G operations, 64
+// operations a byte at 16 sequences with four query heads each, where this chip's matrix pipe does about 240 per byte of memory
+// traffic: read once, the prefix costs its bytes.  One sequence at a time would read it `batch` times.
+// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.3 us (43 MB, 8.5 us at the
+// 5.07 TB/s of a large copy), 32768 + 1024 45.6 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
+// at 16 x 8192.  In its steady state the first launch reads 6.3 TB/s; what is left hardly depends on the lengths: 4 to 5 us until
+// its first tiles are there, 1.5 us at its end, 5 to 6 us for the second launch and the parts in front of it (16.8 MB written and
+// read when 512 workgroups leave some for 16 sequences).
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -56,9 +65,9 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Parts.  A workgroup takes one KV head and one span of cache rows: of the prefix, for the queries of all sequences (batch * G
+// Parts.  A workgroup takes one KV head and runs of its cache rows: of the prefix, for the queries of all sequences (batch * G
 // rows in QT tiles of 32), or of one sequence's own rows, for its G queries.  It leaves, per query row, the reference maximum,
-// the sum and the unnormalised P.V; attn_shared_merge_kernel joins the spans and adds the new token.
+// the sum and the unnormalised P.V; attn_shared_merge_kernel joins the parts and adds the new token.
 //
 // The products are the transposed ones of the prompt pass: S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_32x32x16_f16, so that
 // a lane holds one query's column and the accumulators of the first product are the operand of the second: with the K rows of a
@@ -67,6 +76,10 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 // K and V^T tiles of SK keys travel straight into a ring of LDS stages (buffer_load ... lds); a lane fetches the 16-byte chunk
 // that the bank swizzle assigns to its slot.  The four wavefronts of a workgroup are QT query tiles x KG groups of keys x DH
 // parts of the output dims (DH = 2: both compute the scores, each half of the output).
+//
+// Two workgroups of four wavefronts per compute unit, each with a ring of two 32 KB stages, so that one works or begins while the
+// other waits: 45.3 / 21.0 us at 16 x (32768 + 1024) / (8192 + 256) against 47.8 / 22.8 us with one workgroup of eight
+// wavefronts and four stages.
 // ---------------------------------------------------------------------------------------------------------------
 #define AS_WAVES 4    // wavefronts of a workgroup
 #define AS_THREADS (64 * AS_WAVES)
@@ -96,22 +109,55 @@ template <int HD, int QT, int W> constexpr int as_lds_bytes() {
 }
 
 // Who does what.  The rows of a KV head -- the prefix, then each sequence's own rows -- form one line of units of 64 keys, with
-// AS_START empty units in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the line,
-// whatever the lengths are.  A workgroup leaves one part for each piece of the line that its share touches: part i of the
+// `start` empty units in front of every tail (what starting on it costs), and the workgroups of the head take equal shares of the
+// line, whatever the lengths are.  A workgroup leaves one part for each piece of the line that its share touches: part i of the
 // prefix comes from workgroup i, and workgroup i's part of tail z goes to place i + z (both only grow along the line).
+//
+// Whole tiles: in units of 8, 16 and 32 keys, whose shares are nearer to equal but end inside a tile, 16 x (32768 + 1024) took
+// 47.6, 47.4 and 46.5 us against 45.3, 16 x (8192 + 256) 23.9, 23.6 and 23.3 us against 21.0.
+//
+// A share's size.  A unit costs its workgroup some 1 us as long as memory is not full, a part costs every row of the merge: the
+// best size grows with the square root of the line, and with that of the KV heads, whose parts the merge reads side by side.
+// Measured with 8 heads of 128, shares of 2, 3, 4, 5, 6, 8 and 10 units: 2 x (2048 + 16) 10.9 10.8 11.6 12.4 13.2 14.9 16.6 us,
+// 2 x (4096 + 64) 12.8 11.5 11.8 12.7 13.5 15.2 16.9, 2 x (8192 + 64) 15.0 (3 units at least) 15.0 14.4 13.3 13.8 15.3 17.0,
+// 4 x (16384 + 64) 19.8 (5 at least) .. 20.1 18.0 17.9.  One KV head: 4 x (32768 + 100) 23.0 us with 2 units, 16.0 with 4, 19.7 with
+// 11.  From 16384 positions on all workgroups are wanted, at the smaller heads (half the bytes and less per unit) always: 8 heads of
+// 64, 4 x (32768 + 100) 18.1 us with 8 units, 20.0 with 11.
+//
+// Empty units: 6, 3 where memory is full and a unit takes three times as long: with 3 and 6, 16 x (8192 + 64) 20.0 and 17.2 us,
+// 8 x (8192 + 128) 16.8 and 14.9, 16 x (32768 + 1024) 45.6 and 46.5, 8 x (2048 + 64), in shares of two, 11.6 and 12.4.
 #define AS_UNIT 64
-#define AS_START 3
 struct AsPlan {
-    int wgs, min_share; // workgroups per KV head; units a share has at least
+    int wgs;            // workgroups per KV head
+    uint32_t inv;       // 2^32 / wgs, rounded up
     float *acc, *ml;    // [kvh][wgs][batch * G] of the prefix, then [kvh][wgs + batch][G] of the tails: rows of HD (acc), 2 (ml)
 };
+struct AsShare {
+    int start, share; // empty units in front of a tail, units per workgroup
+};
+template <int HD> __host__ __device__ __forceinline__ AsShare as_share(int prefix_units, int tail_units, int tails, int n_kv_heads, int wgs,
+                                                                             uint32_t inv) {
+    int least = 2;
+    const int size = prefix_units * (n_kv_heads < 8 ? n_kv_heads : 8);
+    if (HD >= 128) {
+#pragma unroll
+        for (int m = 3; m <= 8; ++m) least += size >= 32 * m * m;
+    }
+    AsShare r;
+    r.start = least >= 4 && prefix_units + tail_units + 3 * tails <= 6 * wgs ? 6 : 3;
+    const uint32_t total = (uint32_t)(prefix_units + tail_units + r.start * tails);
+    r.share = wgs > 1 ? (int)((uint64_t)(total + wgs - 1) * inv >> 32) : (int)total; // total / wgs, rounded up
+    if (r.share < least) r.share = least;
+    return r;
+}
 struct AsLine {
     int prefix_units, share, prefix, own_first, lead; // own_first: own row of the first position behind the prefix; lead: rows in
                                                       // front of it in the aligned eight that it lies in
     int tail, first, units;                           // lane z: own rows of sequence z, its first unit, its units
 };
 // Every lane of a wavefront calls it; lane z looks at sequence z.
-template <bool DEV> __device__ __forceinline__ AsLine as_line(const SharedArgs &a, int batch, int wgs, int min_share) {
+template <int HD, bool DEV> __device__ __forceinline__ AsLine as_line(const SharedArgs &a, int n_kv_heads, int batch, int wgs,
+                                                                                 uint32_t inv) {
     const int lane = threadIdx.x % 64;
     const SharedSeq s = shared_seq<DEV>(a, lane < batch ? lane : 0);
     AsLine ln;
@@ -121,16 +167,16 @@ template <bool DEV> __device__ __forceinline__ AsLine as_line(const SharedArgs &
     ln.prefix_units = (ln.prefix + AS_UNIT - 1) / AS_UNIT;
     ln.tail = lane < batch ? s.tail : 0;
     ln.units = ln.tail > 0 ? (ln.lead + ln.tail + AS_UNIT - 1) / AS_UNIT : 0;
-    int end = ln.units > 0 ? ln.units + AS_START : 0; // inclusive sums over the sequences
+    int end = ln.units; // inclusive sums over the sequences
 #pragma unroll
     for (int o = 1; o < LLM_MAX_BATCH; o <<= 1) {
         const int q = __shfl_up(end, o);
         if (lane >= o) end += q;
     }
-    ln.first = ln.prefix_units + end - ln.units;
-    const int total = ln.prefix_units + __builtin_amdgcn_readlane(end, LLM_MAX_BATCH - 1);
-    ln.share = (total + wgs - 1) / wgs;
-    if (ln.share < min_share) ln.share = min_share;
+    const unsigned long long tails = __builtin_amdgcn_ballot_w64(ln.units > 0);
+    const AsShare sh = as_share<HD>(ln.prefix_units, __builtin_amdgcn_readlane(end, LLM_MAX_BATCH - 1), __popcll(tails), n_kv_heads, wgs, inv);
+    ln.share = sh.share;
+    ln.first = ln.prefix_units + end - ln.units + sh.start * __popcll(tails & ((2ull << lane) - 1ull));
     return ln;
 }
 
@@ -348,7 +394,7 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
             issue(st, st + NS);
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // a short span's spare loads
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // a short piece's spare loads
     {
         float lo, hi;
         xhalf(l_run, lo, hi);
@@ -413,14 +459,15 @@ __device__ __forceinline__ void as_part(half_t *smem, const AsPiece &piece, cons
 // Grid: wgs x KV heads, the KV head fastest: consecutive workgroups go round the XCDs, so that a head's queries and tables stay
 // in one XCD's L2.  The arguments in front of `a` are in registers when the kernel starts.
 template <int HD, int G, int QT, bool DEV>
-__global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_shared_part_kernel(float *acc, float *ml, const half_t *qkv, const float *table, int n_kv_heads,
-                                                                      int batch, int wgs, int min_share, int ldq, int prefix_max,
-                                                                      const SharedArgs a) {
+__global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_shared_part_kernel(float *acc, float *ml, const half_t *qkv,
+                                                                                                const float *table, int n_kv_heads, int batch,
+                                                                                                int wgs, uint32_t inv, int ldq, int prefix_max,
+                                                                                                const SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) half_t smem[];
     const int kvh = blockIdx.x % n_kv_heads, wg = blockIdx.x / n_kv_heads;
     const int rows = batch * G;
     const SharedSeq s0 = shared_seq<DEV>(a, 0); // asked for next to the positions that the line needs
-    const AsLine ln = as_line<DEV>(a, batch, wgs, min_share);
+    const AsLine ln = as_line<HD, DEV>(a, n_kv_heads, batch, wgs, inv);
     const int from = wg * ln.share, to = from + ln.share; // this workgroup's units
     if (from < ln.prefix_units) {
         const int end = to * AS_UNIT < ln.prefix ? to * AS_UNIT : ln.prefix;
@@ -454,13 +501,14 @@ __global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_sha
 }
 
 // One workgroup per query head and sequence: the parts' weights (first wavefront) and the new token's score (second one) while
-// the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.
+// the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.  Latency: 4.8 to 6.6 us
+// for 32 heads x 5 to 16 sequences with some 20 to 65 parts each, of which the parts' bytes would take 3.
 #define AS_MERGE_THREADS 256
 // parts per thread asked for at once (80 at head size 128, more than a head of eight has)
 #define AS_MERGE_AHEAD 10
 template <int HD, int G, bool DEV>
 __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(const float *acc, const float *ml, const half_t *qkv, const float *table,
-                                                                             int n_kv_heads, int batch, int wgs, int min_share, int ldq, int max_pos,
+                                                                             int n_kv_heads, int batch, int wgs, uint32_t inv, int ldq, int max_pos,
                                                                              const SharedArgs a) {
     constexpr int LPR = HD / 4, GROUPS = AS_MERGE_THREADS / LPR; // lanes per row of HD floats, rows side by side
     extern __shared__ float weight[]; // one per part
@@ -470,7 +518,7 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
     const int rows = batch * G, Hq = n_kv_heads * G;
     const SharedSeq s = shared_seq<DEV>(a, z);
     const int pos = s.prefix + s.tail, row = s.first + s.tail;
-    const AsLine ln = as_line<DEV>(a, batch, wgs, min_share);
+    const AsLine ln = as_line<HD, DEV>(a, n_kv_heads, batch, wgs, inv);
     const int first = __builtin_amdgcn_readlane(ln.first, z), u = __builtin_amdgcn_readlane(ln.units, z);
     const int np = (ln.prefix_units + ln.share - 1) / ln.share;
     const int w0 = first / ln.share, nt = u > 0 ? (first + u - 1) / ln.share - w0 + 1 : 0, ns = np + nt;
@@ -621,18 +669,29 @@ template <int HD, int G, int QT, bool DEV> static int launch_shared(const Shared
         int rc = llm_ensure_max_smem((const void *)kern, smem, attr_done);
         if (rc != LLM_OK) return rc;
     }
-    // no more workgroups than the longest lengths of the launch give shares to
-    const long long units = (a.max_prefix + AS_UNIT - 1) / AS_UNIT +
-                            (a.max_tail > 0 ? (long long)a.batch * ((a.max_tail + 7 + AS_UNIT - 1) / AS_UNIT + AS_START) : 0);
-    long long used = (units + pl.min_share - 1) / pl.min_share;
+    // no more workgroups than the lengths, or the longest ones that a descriptor may hold, give shares to
+    long long used;
+    if (DEV) {
+        used = ((a.max_prefix + AS_UNIT - 1) / AS_UNIT + (a.max_tail > 0 ? (long long)a.batch * ((a.max_tail + 7 + AS_UNIT - 1) / AS_UNIT + 6) : 0) + 1) / 2;
+    } else {
+        const int prefix_units = (a.max_prefix + AS_UNIT - 1) / AS_UNIT, lead = (a.host.prefix_len - a.host.row0) & 7;
+        int units = 0, tails = 0;
+        for (int z = 0; z < a.batch; ++z) {
+            const int tail = a.host.seq.pos[z] - a.host.prefix_len;
+            units += tail > 0 ? (lead + tail + AS_UNIT - 1) / AS_UNIT : 0;
+            tails += tail > 0;
+        }
+        const AsShare sh = as_share<HD>(prefix_units, units, tails, a.n_kv_heads, pl.wgs, pl.inv);
+        used = (prefix_units + units + sh.start * tails + sh.share - 1) / sh.share;
+    }
     if (used > pl.wgs) used = pl.wgs;
     if (used > 0) {
         kern<<<dim3((unsigned)used * a.n_kv_heads), dim3(AS_THREADS), smem, s>>>(pl.acc, pl.ml, a.qkv, a.table, a.n_kv_heads, a.batch, pl.wgs,
-                                                                                   pl.min_share, a.ldq, a.prefix_max, a);
+                                                                                   pl.inv, a.ldq, a.prefix_max, a);
         LLM_LAUNCH_CHECK("attn_shared_part_kernel");
     }
     attn_shared_merge_kernel<HD, G, DEV><<<dim3(a.n_kv_heads * G, a.batch), dim3(AS_MERGE_THREADS), sizeof(float) * 2 * (pl.wgs + 1), s>>>(
-        pl.acc, pl.ml, a.qkv, a.table, a.n_kv_heads, a.batch, pl.wgs, pl.min_share, a.ldq, a.max_pos, a);
+        pl.acc, pl.ml, a.qkv, a.table, a.n_kv_heads, a.batch, pl.wgs, pl.inv, a.ldq, a.max_pos, a);
     LLM_LAUNCH_CHECK("attn_shared_merge_kernel");
     return LLM_OK;
 }
@@ -652,11 +711,12 @@ template <int HD, int G, bool DEV> static int launch_direct(const SharedArgs &a,
 
 template <int HD, int G> static int launch_shared(const SharedArgs &a, void *ws, hipStream_t s) {
     constexpr int SK = AsShape<HD, 1, AS_DIRECT_WAVES>::SK;
-    if ((a.max_prefix + SK - 1) / SK + (a.max_tail + SK - 1) / SK <= (HD >= 128 ? AS_DIRECT_TILES : AS_DIRECT_TILES + 1)) return a.desc ? launch_direct<HD, G, true>(a, s) : launch_direct<HD, G, false>(a, s);
+    if ((a.max_prefix + SK - 1) / SK + (a.max_tail + SK - 1) / SK <= (HD >= 128 ? AS_DIRECT_TILES : AS_DIRECT_TILES + 1))
+        return a.desc ? launch_direct<HD, G, true>(a, s) : launch_direct<HD, G, false>(a, s);
     const int rows = a.batch * G;
     AsPlan pl = {};
     pl.wgs = as_wgs(a.n_kv_heads);
-    pl.min_share = 2;
+    pl.inv = (uint32_t)(0xffffffffu / pl.wgs + 1);
     pl.acc = (float *)ws;
     pl.ml = pl.acc + (size_t)a.n_kv_heads * ((size_t)pl.wgs * rows + (size_t)(pl.wgs + a.batch) * G) * HD;
     constexpr int MAXR = G * LLM_MAX_BATCH;
