@@ -7,12 +7,17 @@
 // their own, the next segment's loads in flight while one is worked on, and meet at the end of the chunk only; the workgroup of
 // a row that finishes last joins the chunks.
 //
+// What bounds it: many rows, the logits' bytes (read once): 2048 rows of 128256, the best alternative and one given token 96 us,
+// 5.5 TB/s (a large copy reads and writes 5.07); the 20 best 120 us, what listing candidates and cutting the lists adds.  Few
+// rows, latency: 16 rows, 5 best 9.0 us, one row, 20 best 10.7 us, of which an empty launch through the same call is 7; on the
+// chip alone one row takes 5.0 us without alternatives, 8.4 with one and 11 with 20, the two levels of lists.
+//
 // Sums: exponentials are base 2, 2^(x c - R) with c = log2(e) / temperature and R = fl(m c) for the largest logit m so far: one
 // fused operation on the fp16 value, exact before its rounding.  A larger m rescales the lane's sums.  Parts are joined by their
 // R; what the rounding of m c shifted goes out again at the end.
 //
 // The k best (k <= 32) without a sort: the k-th largest of a wavefront's 64 running lane maxima is a lower bound of its k-th
-// largest logit, found by bisection on 16-bit order keys (ballot and bit count, 16 steps).  The few logits from there up are
+// largest logit, found digit by digit on 16-bit order keys (ballots and bit counts, two bits a step).  The few logits from there up are
 // appended to the wavefront's list in LDS; a list that would overflow (many equal logits, rising rows) is cut down to its k
 // best, after which only larger logits can enter, since equal ones further back lose.  A listed logit is a 64-bit word, order
 // key above the complement of its index.
@@ -30,7 +35,9 @@
 #define LP_SLICE 4096          // rows per launch: a counter each at the front of the workspace
 #define LP_LINE 32             // ints from one row's counter to the next: device-scope additions to one line wait for one another
 #define LP_LIST 768            // words of a wavefront's list: a row of 16-byte loads (512 logits) behind what it holds
-#define LP_FEW 3               // lanes above the bound up to which it stays
+// Lanes above the bound up to which it stays, rather than being found anew.  With 0, 3, 8 and 16: 256 rows of 128256, 5 best, 26.5
+// 25.5 28.2 30.3 us, 2048 rows 102.1 101.8 110.4 120.1; 20 best, 700 rows, 57.7 55.6 56.3 61.4.
+#define LP_FEW 3
 #define LP_JOIN (LP_MAX_CHUNKS * LP_MAX_TOP / LP_THREADS) // listed logits per thread when chunks are joined
 #define LP_LOWEST 0x0400u      // order key of -65504, the lowest logit that has a probability
 
@@ -378,7 +385,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
 }
 
 // How a row is cut.  Few rows: finely, so that their logits come from many compute units at once, but into LP_MAX_CHUNKS pieces
-// at most; many rows: coarsely, so that less is joined.
+// at most; many rows: coarsely, so that less is joined.  Aimed at 512 workgroups; with 256, 512 and 1024, rows of 128256: 64 rows,
+// 20 best, 21.2 18.1 17.1 us, 256 rows, 5 best, 28.5 24.6 23.4, but 700 rows, 20 best, 54 54 69.
+// Short chunks in short segments, so that all wavefronts have one, long chunks in long ones with more loads in flight: with 1, 2
+// and 4 loads per lane 16 rows (chunks of 4096) 9.7 9.0 9.3 us, one row (2048) 8.4 and, with 4, 9.3, 2048 whole rows 110 with one
+// and 101 with 4 (5 best).
 struct LpCut {
     int nl, chunk_len, chunks;
 };
