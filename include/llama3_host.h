@@ -211,7 +211,7 @@ void llama3_read_batch_logits(CudaCache *cache0, int b, llm_half *logits);
 
 /* Several answers to one prompt.
  * llama3_fork: dsts[0..n-1] (1..16 caches of the same configuration) become copies of src: its cached rows, ids, position and
- * last logits.  Each stands for itself afterwards and takes every call of this interface; what it held before is gone.  Rows
+ * the logits of the last row that it processed on its own.  Each stands for itself afterwards and takes every call of this interface; what it held before is gone.  Rows
  * that a destination has in common with src from an earlier fork are not copied again, so an answer that branches from its
  * sibling costs its own tokens only.
  * llama3_decode_batch on caches that have rows in common reads those rows once for all sequences
@@ -226,8 +226,8 @@ long llama3_shared_prefix_steps(const CudaCache *c);
  * (0..16; NaN for an id outside the vocabulary), the entropy (pointer may be NULL), the k (0..32) most probable tokens with
  * their log probabilities, largest first, the lowest id first among equals (id -1, -inf where fewer have a probability).  All
  * arrays are host memory, row after row.
- * llama3_logprobs: one row, the last one that c processed.  llama3_batch_logprobs: every sequence of the last
- * llama3_decode_batch with cache0 as caches[0].
+ * llama3_logprobs: one row, the last one that c processed on its own (behind a batched step the call is refused: its rows are
+ * with caches[0]).  llama3_batch_logprobs: every sequence of the last llama3_decode_batch with cache0 as caches[0].
  * llama3_score: llama3_prefill (appends the n tokens, returns the greedy next one) that also rates the text: logprob[i] is that
  * of tokens[i + 1] behind the tokens up to i (NaN for i = n - 1), entropy[i], top_ids/top_logprob[i * k ..] of the same row. */
 void llama3_logprobs(CudaCache *c, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k, int *top_ids,

@@ -144,9 +144,6 @@ __device__ __forceinline__ half8_t load8_nt(const half_t *p) {
     return __builtin_bit_cast(half8_t, v);
 }
 __device__ __forceinline__ void store8(half_t *p, half8_t v) { *reinterpret_cast<half8_t *>(p) = v; }
-__device__ __forceinline__ void store8_nt(half_t *p, half8_t v) {
-    __builtin_nontemporal_store(__builtin_bit_cast(uint4_t, v), reinterpret_cast<uint4_t *>(p));
-}
 
 // RoPE of four adjacent pairs (8 halves): (e, o) -> (c e - s o, s e + c o) with unfused multiplies (the device code
 // is compiled with -ffp-contract=off), each result rounded to fp16.  cs: the four (cos, sin) pairs of the position.

@@ -20,6 +20,10 @@ __device__ __forceinline__ half8_t load8_any(const half_t *p) {
     return v;
 }
 
+__device__ __forceinline__ void store8_nt(half_t *p, half8_t v) { // without keeping the line
+    __builtin_nontemporal_store(__builtin_bit_cast(uint4_t, v), reinterpret_cast<uint4_t *>(p));
+}
+
 // Grid (parts of a head's K + parts of its V, layers * kv heads); a thread takes one 16-byte chunk, aligned at the destination,
 // and stores it to every destination.  K is one contiguous piece per head, V a piece per dim, whose first and last few rows
 // (those that do not fill a chunk) are dealt to the dim's lanes one by one.

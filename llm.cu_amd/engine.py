@@ -203,7 +203,8 @@ class Engine:
         return lp, ent, ti, tl
 
     def logprobs(self, ids=(), k=0, temperature=1.0):
-        """(log probabilities of ids, entropy, top ids, their log probabilities) of the last row processed."""
+        """(log probabilities of ids, entropy, top ids, their log probabilities) of the last row, if it was processed
+        on its own (batch_logprobs has those of batched steps)."""
         lp, ent, ti, tl = self._logprobs(lib().llama3_logprobs, 1, ids, k, temperature)
         return lp[0], float(ent[0]), ti[0], tl[0]
 

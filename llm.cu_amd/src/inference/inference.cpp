@@ -98,6 +98,7 @@ struct Engine {
     llm_graph_t b_graph[17][2] = {};
     bool b_ran[17][2] = {};
     int b_rows = 0; // sequences of the last batched step (rows of b_logits)
+    int logits_pos = 0; // tokens behind the last of which `logits` stands (batched steps leave theirs in b_logits)
     // Rows that other caches hold bit for bit, from llama3_fork: caches with a mark of the same id agree on rows 0 .. len - 1.
     // Marks grow in len; only llama3_cache_reset takes rows back, and with them the marks.
     struct SharedRows {
@@ -460,6 +461,7 @@ int run_pass(Engine *e, const Llama3 *m, const int *tokens, int n, llm_half *log
     e->inject_host = nullptr;
     e->tokens.insert(e->tokens.end(), tokens, tokens + n);
     e->pos += n;
+    e->logits_pos = e->pos;
     // the pass left *d_pos == pos and its pick in d_tokens[pos]
     e->dev_pos_valid = true;
     e->dev_next = e->h_stage[2];
@@ -520,6 +522,7 @@ int step_one(Engine *e, const Llama3 *m, int token, llm_half *logits_host) {
     }
     e->tokens.push_back(token);
     e->pos += 1;
+    e->logits_pos = e->pos;
     e->dev_pos_valid = true;
     e->dev_next = e->h_stage[2];
     return (int)e->h_stage[2];
@@ -765,6 +768,7 @@ extern "C" int *tokens_to_cuda(int *tokens, int embed_size, Tensor *X) {
 extern "C" void llama3_cache_reset(CudaCache *C) {
     Engine *e = eng(C);
     e->pos = 0;
+    e->logits_pos = 0;
     e->tokens.clear();
     e->marks.clear();
     e->dev_pos_valid = false;
@@ -822,6 +826,7 @@ extern "C" int llama3_generate(Llama3 *m, CudaCache *C, const int *prompt, int n
     // host mirror: the decode steps consumed out_tokens[0..n_decode-2]
     for (int i = 0; i + 1 < n_decode; ++i) e->tokens.push_back(out_tokens[i]);
     e->pos += n_decode - 1;
+    e->logits_pos = e->pos;
     e->dev_pos_valid = true; // every replayed step advanced *d_pos and stored its pick at d_tokens[pos]
     e->dev_next = out_tokens[n_decode - 1];
     if (stats) {
@@ -981,6 +986,7 @@ extern "C" void llama3_fork(CudaCache *src, CudaCache *const *dsts, int n) {
     for (int i = 0; i < n; ++i) {
         es[i]->tokens = e->tokens;
         es[i]->pos = e->pos;
+        es[i]->logits_pos = e->logits_pos;
         es[i]->marks = e->marks;
         es[i]->dev_pos_valid = false; // its device copies of position and ids are those of what it held before
         es[i]->dev_next = -1;
@@ -1000,6 +1006,7 @@ extern "C" void llama3_logprobs(CudaCache *C, float temperature, const int *ids,
     Engine *e = eng(C);
     check_logprob_args(e, n_ids, k, ids, logprob, top_ids, top_logprob);
     if (e->pos == 0) llama3_fail("llama3_logprobs: no row has been processed");
+    if (e->logits_pos != e->pos) llama3_fail("llama3_logprobs: the last row was a batched step's (llama3_batch_logprobs)");
     logprob_rows(e, e->logits, 1, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
 }
 

@@ -247,6 +247,30 @@ def test_answers_command(gpu):
     assert "batched steps that read the prompt's rows once: 4 of 4" in p.stdout
 
 
+BATCHED = "a.prefill([1]); b.prefill([2]); E = pkg.engine.Engine; E.decode_batch([a, b], [3, 4]); "
+
+
+def test_log_probabilities_behind_a_batched_step(tiny):
+    """A step of a cache's own behind a batched one makes the last row its own again, in a fork of it too."""
+    gpu, cfg, model = tiny
+    a, b = engines(gpu, cfg, model, 2)
+    a.prefill([5, 6, 7])
+    a.fork([b])
+    gpu.engine.Engine.decode_batch([a, b], [8, 9])
+    a.decode(10)
+    a.fork([b])
+    ids = [1, 2, 3]
+    of_a, of_b = a.logprobs(ids, 5), b.logprobs(ids, 5)
+    assert all(np.array_equal(p, q) for p, q in zip(of_a, of_b))
+    check_logprobs(a.logits(), 1.0, ids, 5, of_a)
+    close_all([a, b])
+
+
+@pytest.mark.parametrize("code", ["a.logprobs([1])", "b.logprobs([1])", "c = E(m, cfg); b.fork([c]); c.logprobs([1])"])
+def test_log_probabilities_of_a_batched_row_are_refused(gpu, code):
+    test_refusals_end_with_a_message(gpu, BATCHED + code, "batched step")
+
+
 REFUSALS = [
     ("a.fork([])", "destinations"), ("a.fork([a])", "is the source"), ("a.fork([b, b])", "share a cache"),
     ("a.fork([pkg.engine.Engine(m, pkg.engine.config('tiny', max_pos=128))])", "different configuration"),
