@@ -9,8 +9,8 @@
 // What bounds it: the bytes of the caches.  Per KV head and prefix position 2 hd halves are read for 4 hd batch G operations, 64
 // operations a byte at 16 sequences with four query heads each, where this chip's matrix pipe does about 240 per byte of memory
 // traffic: read once, the prefix costs its bytes.  One sequence at a time would read it `batch` times.
-// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.3 us (43 MB, 8.5 us at the
-// 5.07 TB/s of a large copy), 32768 + 1024 45.6 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
+// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.2 us (43 MB, 8.5 us at the
+// 5.07 TB/s of a large copy), 32768 + 1024 45.5 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
 // at 16 x 8192.  In its steady state the first launch reads 6.3 TB/s; what is left hardly depends on the lengths: 4 to 5 us until
 // its first tiles are there, 1.5 us at its end, 5 to 6 us for the second launch and the parts in front of it (16.8 MB written and
 // read when 512 workgroups leave some for 16 sequences).
@@ -167,12 +167,14 @@ template <int HD, bool DEV> __device__ __forceinline__ AsLine as_line(const Shar
     ln.prefix_units = (ln.prefix + AS_UNIT - 1) / AS_UNIT;
     ln.tail = lane < batch ? s.tail : 0;
     ln.units = ln.tail > 0 ? (ln.lead + ln.tail + AS_UNIT - 1) / AS_UNIT : 0;
-    int end = ln.units; // inclusive sums over the sequences
-#pragma unroll
-    for (int o = 1; o < LLM_MAX_BATCH; o <<= 1) {
-        const int q = __shfl_up(end, o);
-        if (lane >= o) end += q;
-    }
+    // inclusive sums over the sequences, the first row of 16 lanes (row_shr by 1, 2, 4, 8; zeros come in): a chain in front of every
+    // load, 0.1 to 0.3 us of both launches shorter than by shuffles
+    int end = ln.units;
+    static_assert(LLM_MAX_BATCH == 16, "one row of lanes");
+    end += __builtin_amdgcn_update_dpp(0, end, 0x111, 0xf, 0xf, true);
+    end += __builtin_amdgcn_update_dpp(0, end, 0x112, 0xf, 0xf, true);
+    end += __builtin_amdgcn_update_dpp(0, end, 0x114, 0xf, 0xf, true);
+    end += __builtin_amdgcn_update_dpp(0, end, 0x118, 0xf, 0xf, true);
     const unsigned long long tails = __builtin_amdgcn_ballot_w64(ln.units > 0);
     const AsShare sh = as_share<HD>(ln.prefix_units, __builtin_amdgcn_readlane(end, LLM_MAX_BATCH - 1), __popcll(tails), n_kv_heads, wgs, inv);
     ln.share = sh.share;
