@@ -9,8 +9,8 @@
 //
 // What bounds it: many rows, the logits' bytes (read once): 2048 rows of 128256, the best alternative and one given token 96 us,
 // 5.5 TB/s (a large copy reads and writes 5.07); the 20 best 120 us, what listing candidates and cutting the lists adds.  Few
-// rows, latency: 16 rows, 5 best 9.0 us, one row, 20 best 10.7 us, of which an empty launch through the same call is 7; on the
-// chip alone one row takes 5.0 us without alternatives, 8.4 with one and 11 with 20, the two levels of lists.
+// rows, latency: 16 rows, 5 best 8.6 us, one row, 20 best 10.1 us, of which an empty launch through the same call is 7; on the
+// chip alone one row takes 5.0 us without alternatives, some 5 more with 20: the two levels of lists.
 //
 // Sums: exponentials are base 2, 2^(x c - R) with c = log2(e) / temperature and R = fl(m c) for the largest logit m so far: one
 // fused operation on the fp16 value, exact before its rounding.  A larger m rescales the lane's sums.  Parts are joined by their
@@ -183,16 +183,38 @@ __device__ __forceinline__ void lp_cut(lp_word *list, int n, int k) {
     lp_wave_sync();
 }
 
-// The wavefronts' lists (k words each, cut) into best, largest first.  All threads call it, behind a barrier.
-__device__ __forceinline__ void lp_join_waves(const lp_word *lists, int k, lp_word *best) {
+// A wavefront's list made ready for lp_join_waves: cut unless it is hardly longer than k (joining costs every word of it four times
+// what cutting does), and a multiple of eight with zeros.  Returns its length, at most 64.
+__device__ __forceinline__ int lp_ready(lp_word *list, int n, int k) {
+    if (n > k + 8) {
+        lp_cut(list, n, k);
+        n = k; // zeros in the place of what is missing
+    }
+    const int lane = threadIdx.x % 64, n8 = (n + 7) & ~7;
+    if (lane < n8 - n) list[n + lane] = 0ull;
+    return n8;
+}
+
+// The wavefronts' lists (n8[w] words each) into best, largest first.  All threads call it, behind a barrier.
+__device__ __forceinline__ void lp_join_waves(const lp_word *lists, const int *n8, int k, lp_word *best) {
+    static_assert(LP_MAX_TOP + 8 <= 64, "a word per thread");
     const int tid = threadIdx.x;
+    int size[LP_WAVES], from = 0; // the first threads take a word each
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; ++w) size[w] = n8[w];
     if (tid < k) best[tid] = 0ull;
     __syncthreads();
-    if (tid < LP_WAVES * k) {
-        const lp_word mine = lists[tid / k * LP_LIST + tid % k];
+    int at = -1;
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; ++w) {
+        if (tid >= from && tid < from + size[w]) at = w * LP_LIST + tid - from;
+        from += size[w];
+    }
+    if (at >= 0) {
+        const lp_word mine = lists[at];
         int rank = 0;
 #pragma unroll
-        for (int w = 0; w < LP_WAVES; ++w) rank += lp_rank(lists + w * LP_LIST, (k + 7) & ~7, mine);
+        for (int w = 0; w < LP_WAVES; ++w) rank += lp_rank(lists + w * LP_LIST, size[w], mine);
         if (mine && rank < k) best[rank] = mine;
     }
     __syncthreads();
@@ -205,7 +227,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     extern __shared__ __attribute__((aligned(16))) lp_word lists[]; // LP_WAVES lists of LP_LIST words when k > 0
     __shared__ lp_word best[LP_MAX_TOP];
     __shared__ float part[LP_WAVES][3];
-    __shared__ int is_last;
+    __shared__ int is_last, ready[LP_WAVES];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunk = blockIdx.x, k = a.k;
     const size_t row = blockIdx.y;
     const half_t *x = a.x + row * a.ld;
@@ -308,7 +330,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         part[wave][1] = st.s;
         part[wave][2] = st.t;
     }
-    if (k > 0) lp_cut(list, n, k);
+    if (k > 0) {
+        const int n8 = lp_ready(list, n, k);
+        if (lane == 0) ready[wave] = n8;
+    }
     __syncthreads();
     float M = part[0][0];
 #pragma unroll
@@ -320,7 +345,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         st.s += p.s;
         st.t += p.t;
     }
-    if (k > 0) lp_join_waves(lists, k, best);
+    if (k > 0) lp_join_waves(lists, ready, k, best);
     // ---- 3. several chunks: leave this one's result; the row's last workgroup goes on -------------------------------------
     if (a.chunks > 1) {
         // Handed over by device-scope stores (written through to where every XCD reads them) that are complete before the
@@ -361,9 +386,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
                 const unsigned long long who = __builtin_amdgcn_ballot_w64(mine_too);
                 if (who) n = lp_append(list, n, who, mine_too, w[j]);
             }
-            lp_cut(list, n, k);
+            const int n8 = lp_ready(list, n, k);
+            if (lane == 0) ready[wave] = n8;
             __syncthreads();
-            lp_join_waves(lists, k, best);
+            lp_join_waves(lists, ready, k, best);
         }
     }
     // ---- 4. results ------------------------------------------------------------------------------------------------------
