@@ -131,7 +131,7 @@ constexpr int ROPE_IN_ATTENTION_FROM = 4096;
 // Batched steps of forks read the shared prefix once for all from this many shared positions on, and where batch times
 // positions makes up for the second launch.  Measured, attention of a layer (8B heads), every cache for itself against shared:
 // 2 sequences, 1024 positions 10.3 against 11.8 us, 2048 12.8 against 12.1; 4 sequences, 512 10.7 against 11.9, 1024 12.8 against
-// 11.9; 8 sequences, 512 14.5 against 12.0; 16 sequences, 256 11.9 against 13.8, 512 21.7 against 14.2, 8192 108 against 21.5.
+// 11.9; 8 sequences, 512 14.5 against 12.0; 16 sequences, 256 11.9 against 13.8, 512 21.8 against 14.0, 8192 108 against 18.2.
 constexpr int SHARED_FROM = 512, SHARED_FROM_ROWS = 4096;
 constexpr size_t MAX_MARKS = 8;
 constexpr int LP_ROWS = 512; // rows of logits that llama3_score holds at a time
