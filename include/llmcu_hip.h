@@ -281,7 +281,8 @@ int llm_attn_decode_rope_batch_dev(const uint16_t *qkv_dev, int ldq, const llm_b
  * (with row0 = 0 and prefix_max_pos = max_pos); own caches are distinct.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
  * 2 GiB.  Rows that hold no position yet may hold anything, NaN included.
  * Arithmetic: queries and the new key are rounded to fp16 after the rotation (llm_rope's results), products on the matrix
- * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32.  The order of the sums depends on the
+ * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32; a softmax weight is the sum of two fp16
+ * operands, within 2^-22 of itself and 2^-32 of the largest.  The order of the sums depends on the
  * lengths only: equal calls give equal bits.
  * workspace: llm_attn_shared_workspace_bytes, zeroed once with llm_fill_zero before its first use (every call leaves it
  * reusable, by calls of other shapes too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured graphs.

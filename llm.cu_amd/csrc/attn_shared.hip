@@ -6,11 +6,11 @@
 // Positions 0..prefix_len-1 come from one prefix cache, positions prefix_len..p_z-1 from the sequence's own cache (row r
 // holds position row0 + r), position p_z is the new token, whose rotated key and value are appended to the own cache.
 //
-// What bounds it: the bytes of the caches.  Per KV head and prefix position 2 hd halves are read for 4 hd batch G operations, 64
-// operations a byte at 16 sequences with four query heads each, where this chip's matrix pipe does about 240 per byte of memory
-// traffic: read once, the prefix costs its bytes.  One sequence at a time would read it `batch` times.
-// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.2 us (43 MB, 8.5 us at the
-// 5.07 TB/s of a large copy), 32768 + 1024 45.5 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
+// What bounds it: the bytes of the caches.  Per KV head and prefix position 2 hd halves are read for 4 hd batch G operations (6 hd
+// with the second half of the weights), 64 (96) operations a byte at 16 sequences with four query heads each, where this chip's
+// matrix pipe does about 240 per byte of memory traffic: read once, the prefix costs its bytes.  One sequence at a time would read it `batch` times.
+// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.4 us (43 MB, 8.5 us at the
+// 5.07 TB/s of a large copy), 32768 + 1024 46.4 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
 // at 16 x 8192.  In its steady state the first launch reads 6.3 TB/s; what is left hardly depends on the lengths: 4 to 5 us until
 // its first tiles are there, 1.5 us at its end, 5 to 6 us for the second launch and the parts in front of it (16.8 MB written and
 // read when 512 workgroups leave some for 16 sequences).
@@ -300,6 +300,8 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
         for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
     float m_run = -FLT_MAX, l_run = 0.f;
     const float c2 = 1.44269504088896341f / sqrtf((float)HD);
+    float minus = -1.f;
+    asm("" : "+v"(minus)); // not folded: a multiplication, so that conversion, difference and rounding are one instruction
     const int pm = (n & ~0xC) | ((n & 8) >> 1) | ((n & 4) << 1); // pi(n)
     auto xhalf = [](float x, float &lo, float &hi) {
         auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -354,16 +356,16 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
                     s[e] = key >= r_lo && key < r_hi ? s[e] : -FLT_MAX;
                 }
             }
-            // The reference of the exponentials moves when a score leaves it behind by 2^8: probabilities stay below 2^8 in
-            // fp16 (their relative rounding does not depend on the reference), sums and output are fp32, and O^T is
-            // rescaled a handful of times.
+            // The reference of the exponentials lies 7 below the largest score when it is set and moves when a score leaves it
+            // behind by 15, so that O^T is rescaled a handful of times: weights stay below 2^15, inside fp16, and the best ones
+            // above 2^7, which leaves 2^-32 of them for the finest step of the type.
             float mx = -FLT_MAX, lo, hi;
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
             xhalf(mx, lo, hi);
             mx = fmaxf(lo, hi) * c2;
-            if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.f)) {
-                const float m_new = mx > m_run + 8.f ? mx : m_run, alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            if (__builtin_amdgcn_ballot_w64(mx > m_run + 15.f)) {
+                const float m_new = mx > m_run + 15.f ? mx - 7.f : m_run, alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 l_run *= alpha;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -371,15 +373,20 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
                     for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
                 m_run = m_new;
             }
-            // probabilities rounded to fp16, the operand type of the second product; their sum is that of the rounded ones, so
-            // that numerator and denominator use the same weights
-            half8_t p[2];
+            // The operands of the second product are fp16: a weight goes in as the sum of two of them, off by 2^-22 of itself at most,
+            // or 2^-25, half the type's finest step.  In one (2^-11) the result was off by 2.4 to 2.9e-4 of its size; the fp16
+            // result's own rounding is 2.1e-4.  16 x (8192 + 256) 18.2 -> 18.4 us, 16 x (32768 + 1024) 45.4 -> 46.4, 5 x (5003 + 77) 14.0 -> 14.7.
+            half8_t p[2], q[2];
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const half2_t h = {(half_t)__builtin_amdgcn_exp2f(fmaf(s[e], c2, -m_run)), (half_t)__builtin_amdgcn_exp2f(fmaf(s[e + 1], c2, -m_run))};
+                const float w0 = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m_run)), w1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c2, -m_run));
+                l_run += w0 + w1;
+                half2_t h = {(half_t)w0, (half_t)w1};
+                asm("" : "+v"(h)); // both uses take the converted pair
                 p[e / 8][e % 8] = h[0];
                 p[e / 8][e % 8 + 1] = h[1];
-                l_run = __builtin_amdgcn_fdot2(h, half2_t{(half_t)1.f, (half_t)1.f}, l_run, false);
+                q[e / 8][e % 8] = (half_t)fmaf((float)h[0], minus, w0); // exact before its rounding
+                q[e / 8][e % 8 + 1] = (half_t)fmaf((float)h[1], minus, w1);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -388,6 +395,7 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
                     const int dim = 32 * (dh * DT + t) + n;
                     const half8_t vf = load8(vs_ + dim * SK + ((kc / 8 + 2 * u + hb) ^ swz(dim, NCV)) * 8);
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[u], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q[u], o[t], 0, 0, 0);
                 }
             }
         }
@@ -656,9 +664,9 @@ __global__ __launch_bounds__(64 * AS_DIRECT_WAVES) void attn_shared_direct_kerne
 }
 
 // Tiles (128 keys at head size 128, 256 at the others) up to which that is faster than two launches, one more at the smaller
-// head sizes.  Measured on 1, 4 and 16 sequences, direct against parts: head size 128, three tiles 9.3 / 9.3 / 9.5 against 10.8 /
-// 10.8 / 13.3 us, five 11.9 / 12.0 / 12.1 against 10.8 / 10.8 / 13.5; head size 64, five 10.2 / 10.3 / 10.4 against 10.7, nine 15.3
-// against 10.7; head size 32, five 7.9 / 8.1 / 8.1 against 10.7.
+// head sizes.  Measured on 1, 4 and 16 sequences, direct against parts: head size 128, four tiles 10.5 / 10.6 / 10.8 against 10.8 /
+// 10.8 / 12.7 us, five 11.9 / 12.0 / 12.1 against 10.8 / 10.8 / 12.7; head size 64, five 10.5 / 10.6 / 10.6 against 10.8 / 10.8 / 10.9,
+// six 11.8 / 11.9 / 11.9 against 10.8 / 10.8 / 10.9; head size 32, five 8.4 / 8.6 / 8.7 against 10.8.
 #define AS_DIRECT_TILES 4
 // Workgroups per KV head: two on each of the 256 compute units.
 static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 * AS_PER_CU ? 256 * AS_PER_CU / n_kv_heads : 1; }

@@ -296,3 +296,66 @@ def test_captured_step_follows_the_descriptor(gpu):
         state["kcs"], state["vcs"] = got[1], got[2]
     check(L.llm_graph_destroy(graph))
     check(L.llm_stream_destroy(stream))
+
+
+def closely(c):
+    """expected() with the tolerance of weights that enter the second product as the sum of two fp16 values.  Per element, with
+    u = 2^-24, n the positions, size the largest sum |q k| / sqrt(head_dim), which bounds every score:
+      half an fp16 step of the result, 2^-11 |o| + 2^-25
+      the second product's weights: the first part rounded to 11 bits, the rest (2^-11 of the weight at most) too: 2^-22, relative,
+        and 2^-25 of a scale on which the largest weight is 2^7 or more: n 2^-32 max |v|
+      exp2: two units of the last place, 4 u; its argument: accumulation and scaling of the score (head_dim + 2) size u, three
+        roundings of the factor 3 size u, one of the difference to the reference, whose value is below 2 size log2 e + 16, and
+        two more of that kind where references are joined: 3 (2 size + 12) u
+      sums of weights and of weighted values, in any order: n u
+    all but the first two of them once in the numerator and once in the denominator."""
+    out, _, kcs, vcs = expected(c)
+    Hq, Hkv, hd = c["heads"]
+    G, P, row0 = Hq // Hkv, c["prefix"], c["row0"]
+    tol, u = np.zeros_like(out), 2.0 ** -24
+    for z, pos in enumerate(c["positions"]):
+        q = H.f16(orc.rope(np.ascontiguousarray(c["qkv"][z:z + 1, :Hq * hd]), Hq, hd, pos)).reshape(Hq, hd)
+        for h in range(Hkv):
+            K = np.concatenate([H.f16(c["kp"][h, :P]), H.f16(kcs[z, h, P - row0:pos - row0 + 1])])
+            V = np.abs(np.concatenate([H.f16(c["vp"][h, :, :P]).reshape(hd, P), H.f16(vcs[z, h, :, P - row0:pos - row0 + 1])], 1))
+            n = pos + 1
+            for g in range(h * G, (h + 1) * G):
+                s = K @ q[g] / np.sqrt(hd)
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                size = (np.abs(K) @ np.abs(q[g])).max() / np.sqrt(hd)
+                rel = 2.0 ** -22 + 2 * u * (4 + (hd + 2) * size + 3 * size + 3 * (2 * size + 12) + n)
+                at = slice(g * hd, (g + 1) * hd)
+                tol[z, at] = 2.0 ** -11 * np.abs(out[z, at]) + 2.0 ** -25 + rel * (V @ w) + n * 2.0 ** -32 * V.max() * w.max()
+    return out, tol, kcs, vcs
+
+
+@pytest.mark.parametrize("heads", SHAPES)
+@pytest.mark.parametrize("prefix", [90, 1500])
+def test_weights_are_held_in_more_than_the_operands_type(gpu, heads, prefix):
+    """Few positions of like weight and values of either sign: a weight in a single fp16 shows beside the result's rounding."""
+    c = case(31, 4, prefix, [0, 17, 70, 33], heads, False, scale=1.5)
+    say("weights", heads, prefix)
+    verify(run(gpu, c), closely(c))
+
+
+@pytest.mark.parametrize("gap", [6, 10, 14, 18, 22, 25, 28, 31])
+@pytest.mark.parametrize("n", [120, 6000])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 1, 64), (2, 2, 32)])
+def test_many_small_weights_count(gpu, heads, n, gap):
+    """One position far ahead of n others, each 2^-gap of its weight: together they are a part of the result at any gap."""
+    Hq, Hkv, hd = heads
+    c = case(32, 2, n, [0, 3], heads, False)
+    q = np.tile(np.random.default_rng(gap).standard_normal(hd), Hq)
+    for z in range(2):
+        c["qkv"][z, :Hq * hd] = H.bits(q)
+        c["qkv"][z, Hq * hd:(Hq + Hkv) * hd] = 0                    # the new key: score 0
+        c["qkv"][z, (Hq + Hkv) * hd:] = H.bits(1.0)
+    turned = H.f16(orc.rope(np.ascontiguousarray(c["qkv"][:1, :Hq * hd]), Hq, hd, n)).reshape(Hq, hd)[0]
+    c["kp"][:, :n], c["vp"][:, :, :n] = 0, H.bits(1.0)
+    c["kcs"][1, :, n:n + 3], c["vcs"][1, :, :, n:n + 3] = 0, H.bits(1.0)
+    ahead = n // 3
+    c["kp"][:, ahead] = H.bits(turned * (gap * np.log(2.0) * np.sqrt(hd) / (turned @ turned)))
+    c["vp"][:, :, ahead] = 0
+    say("gap", gap, "of", n, heads)
+    verify(run(gpu, c), closely(c))
