@@ -9,8 +9,8 @@
 // What bounds it: the bytes of the caches.  Per KV head and prefix position 2 hd halves are read for 4 hd batch G operations (6 hd
 // with the second half of the weights), 64 (96) operations a byte at 16 sequences with four query heads each, where this chip's
 // matrix pipe does about 240 per byte of memory traffic: read once, the prefix costs its bytes.  One sequence at a time would read it `batch` times.
-// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.4 us (43 MB, 8.5 us at the
-// 5.07 TB/s of a large copy), 32768 + 1024 46.4 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
+// Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.5 us (43 MB, 8.5 us at the
+// 5.07 TB/s of a large copy), 32768 + 1024 46.6 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
 // at 16 x 8192.  In its steady state the first launch reads 6.3 TB/s; what is left hardly depends on the lengths: 4 to 5 us until
 // its first tiles are there, 1.5 us at its end, 5 to 6 us for the second launch and the parts in front of it (16.8 MB written and
 // read when 512 workgroups leave some for 16 sequences).
@@ -188,6 +188,9 @@ struct AsPiece {
     int max_pos, begin, lo, hi;
 };
 
+// References of exponentials are unscaled scores; as_c2 takes a difference of two to the base of exp2.
+template <int HD> __device__ __forceinline__ float as_c2() { return 1.44269504088896341f / sqrtf((float)HD); }
+
 // The tiles of NP pieces, one behind the other, for up to 32 QT query rows.
 // q_row(r): query row r, not rotated (any r below 32 QT); q_seq(r): which of the staged rows cs_row(i), i < LLM_MAX_BATCH, of the
 // (cos, sin) table is its position's.
@@ -299,7 +302,7 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
     float m_run = -FLT_MAX, l_run = 0.f;
-    const float c2 = 1.44269504088896341f / sqrtf((float)HD);
+    const float c2 = as_c2<HD>();
     float minus = -1.f;
     asm("" : "+v"(minus)); // not folded: a multiplication, so that conversion, difference and rounding are one instruction
     const int pm = (n & ~0xC) | ((n & 8) >> 1) | ((n & 4) << 1); // pi(n)
@@ -356,16 +359,16 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
                     s[e] = key >= r_lo && key < r_hi ? s[e] : -FLT_MAX;
                 }
             }
-            // The reference of the exponentials lies 7 below the largest score when it is set and moves when a score leaves it
-            // behind by 15, so that O^T is rescaled a handful of times: weights stay below 2^15, inside fp16, and the best ones
+            // The reference of the exponentials lies 7 (in their base 2) below the largest score when it is set and moves when a score
+            // leaves it behind by 15, so that O^T is rescaled a handful of times: weights stay below 2^15, inside fp16, and the best ones
             // above 2^7, which leaves 2^-32 of them for the finest step of the type.
             float mx = -FLT_MAX, lo, hi;
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
             xhalf(mx, lo, hi);
-            mx = fmaxf(lo, hi) * c2;
-            if (__builtin_amdgcn_ballot_w64(mx > m_run + 15.f)) {
-                const float m_new = mx > m_run + 15.f ? mx - 7.f : m_run, alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            mx = fmaxf(lo, hi);
+            if (__builtin_amdgcn_ballot_w64(mx - m_run > 15.f / c2)) {
+                const float m_new = mx - m_run > 15.f / c2 ? mx - 7.f / c2 : m_run, alpha = __builtin_amdgcn_exp2f((m_run - m_new) * c2);
                 l_run *= alpha;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -373,29 +376,35 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
                     for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
                 m_run = m_new;
             }
+            // The difference to the reference comes first, then the scaling: with one fused operation on scaled scores every exponent
+            // is off by the rounding of the reference, which takes the weights out of fp16 where scores pass 10^7 (and is no
+            // faster: 11.6 against 11.2 us at 7 x (1023 + 1), 18.5 and 18.5 at 16 x (8192 + 256)).
             // The operands of the second product are fp16: a weight goes in as the sum of two of them, off by 2^-22 of itself at most,
             // or 2^-25, half the type's finest step.  In one (2^-11) the result was off by 2.4 to 2.9e-4 of its size; the fp16
-            // result's own rounding is 2.1e-4.  16 x (8192 + 256) 18.2 -> 18.4 us, 16 x (32768 + 1024) 45.4 -> 46.4, 5 x (5003 + 77) 14.0 -> 14.7.
-            half8_t p[2], q[2];
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float w0 = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m_run)), w1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c2, -m_run));
-                l_run += w0 + w1;
-                half2_t h = {(half_t)w0, (half_t)w1};
-                asm("" : "+v"(h)); // both uses take the converted pair
-                p[e / 8][e % 8] = h[0];
-                p[e / 8][e % 8 + 1] = h[1];
-                q[e / 8][e % 8] = (half_t)fmaf((float)h[0], minus, w0); // exact before its rounding
-                q[e / 8][e % 8 + 1] = (half_t)fmaf((float)h[1], minus, w1);
-            }
+            // result's own rounding is 2.1e-4.  16 x (8192 + 256) 18.2 -> 18.4 us, 16 x (32768 + 1024)
+            // 45.4 -> 46.4, 5 x (5003 + 77) 14.0 -> 14.7.
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f((s[8 * u + e] - m_run) * c2);
+                half8_t p, q;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    l_run += w[e] + w[e + 1];
+                    half2_t h = {(half_t)w[e], (half_t)w[e + 1]};
+                    asm("" : "+v"(h)); // both uses take the converted pair
+                    p[e] = h[0];
+                    p[e + 1] = h[1];
+                    q[e] = (half_t)fmaf((float)h[0], minus, w[e]); // exact before its rounding
+                    q[e + 1] = (half_t)fmaf((float)h[1], minus, w[e + 1]);
+                }
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const int dim = 32 * (dh * DT + t) + n;
                     const half8_t vf = load8(vs_ + dim * SK + ((kc / 8 + 2 * u + hb) ^ swz(dim, NCV)) * 8);
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[u], o[t], 0, 0, 0);
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q[u], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p, o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q, o[t], 0, 0, 0);
                 }
             }
         }
@@ -423,8 +432,7 @@ __device__ __forceinline__ void as_tiles(half_t *smem, const AsPiece (&pc)[NP], 
     __syncthreads();
 }
 
-// What as_tiles left for dims 4 d4 .. + 3 of a query row: the groups of keys joined (unnormalised), the row's maximum (base 2)
-// and sum.
+// What as_tiles left for dims 4 d4 .. + 3 of a query row: the groups of keys joined (unnormalised), the row's reference and sum.
 template <int HD, int QT, int W>
 __device__ __forceinline__ float4_t as_result(const half_t *smem, int row, int d4, float &m, float &l) {
     using S = AsShape<HD, QT, W>;
@@ -443,7 +451,7 @@ __device__ __forceinline__ float4_t as_result(const half_t *smem, int row, int d
     l = 0.f;
 #pragma unroll
     for (int g = 0; g < S::KG; ++g) {
-        const float f = __builtin_amdgcn_exp2f(ml[g][0] - m); // 0 for a group without a key
+        const float f = __builtin_amdgcn_exp2f((ml[g][0] - m) * as_c2<HD>()); // 0 for a group without a key
         const float4_t x = *reinterpret_cast<const float4_t *>(base + g * QT * PER + ((4 * t + e4) * AS_BLOCK + n + AS_HALF * (d4 % 2)) * 4);
         l += f * ml[g][1];
 #pragma unroll
@@ -526,6 +534,7 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
     __shared__ float4_t part[GROUPS][LPR];
     const int h = blockIdx.x, z = blockIdx.y, kvh = h / G, g = h % G, tid = threadIdx.x, lane = tid % 64;
     const int rows = batch * G, Hq = n_kv_heads * G;
+    const float c2 = as_c2<HD>();
     const SharedSeq s = shared_seq<DEV>(a, z);
     const int pos = s.prefix + s.tail, row = s.first + s.tail;
     const AsLine ln = as_line<HD, DEV>(a, n_kv_heads, batch, wgs, inv);
@@ -550,13 +559,13 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
             const float2_t p = *reinterpret_cast<const float2_t *>(ml + 2 * slot(i));
             // relative to this lane's largest so far
             const float m = fmaxf(M, p[0]);
-            l = l * __builtin_amdgcn_exp2f(M - m) + p[1] * __builtin_amdgcn_exp2f(p[0] - m);
+            l = l * __builtin_amdgcn_exp2f((M - m) * c2) + p[1] * __builtin_amdgcn_exp2f((p[0] - m) * c2);
             M = m;
             weight[i] = p[0];
         }
         const float all = wave_max(M);
-        l = wave_sum(l * __builtin_amdgcn_exp2f(M - all));
-        for (int i = lane; i < ns; i += 64) weight[i] = __builtin_amdgcn_exp2f(weight[i] - all);
+        l = wave_sum(l * __builtin_amdgcn_exp2f((M - all) * c2));
+        for (int i = lane; i < ns; i += 64) weight[i] = __builtin_amdgcn_exp2f((weight[i] - all) * c2);
         if (lane == 0) {
             m_parts = all;
             l_parts = l;
@@ -575,7 +584,7 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
                 for (int e = 0; e < 8; ++e) s.vc[((size_t)kvh * HD + lane * 8 + e) * max_pos + row] = vv[e];
             }
         }
-        dot = wave_sum(dot) * (1.44269504088896341f / sqrtf((float)HD));
+        dot = wave_sum(dot);
         if (lane == 0) m_new = dot;
     }
     __syncthreads();
@@ -596,7 +605,7 @@ __global__ __launch_bounds__(AS_MERGE_THREADS) void attn_shared_merge_kernel(con
     part[grp][d4] = o;
     __syncthreads();
     if (tid < LPR) {
-        const float M = fmaxf(m_parts, m_new), f = __builtin_amdgcn_exp2f(m_parts - M), w = __builtin_amdgcn_exp2f(m_new - M);
+        const float M = fmaxf(m_parts, m_new), f = __builtin_amdgcn_exp2f((m_parts - M) * c2), w = __builtin_amdgcn_exp2f((m_new - M) * c2);
         const float inv = 1.0f / (f * l_parts + w);
         const half4_t x = *reinterpret_cast<const half4_t *>(vn + 4 * d4);
         half_t *out = a.out + (size_t)z * a.ldo + (size_t)h * HD + 4 * d4;
@@ -650,8 +659,7 @@ __global__ __launch_bounds__(64 * AS_DIRECT_WAVES) void attn_shared_direct_kerne
         if (d4 < HD / 8) dot = dot8(load8(q_rot + h * HD + 8 * d4), load8(k_new + 8 * d4), 0.f);
 #pragma unroll
         for (int x = LANES / 2; x >= 1; x /= 2) dot += __shfl_xor(dot, x);
-        dot *= 1.44269504088896341f / sqrtf((float)HD);
-        const float M = fmaxf(m, dot), f = __builtin_amdgcn_exp2f(m - M), w = __builtin_amdgcn_exp2f(dot - M), inv = 1.0f / (f * l + w);
+        const float M = fmaxf(m, dot), f = __builtin_amdgcn_exp2f((m - M) * as_c2<HD>()), w = __builtin_amdgcn_exp2f((dot - M) * as_c2<HD>()), inv = 1.0f / (f * l + w);
         half_t *row = out + (size_t)z * ldo + (size_t)(kvh * G + h) * HD + 4 * d4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) row[e] = (half_t)((f * o[e] + w * (float)v_new[e]) * inv);

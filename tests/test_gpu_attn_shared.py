@@ -17,6 +17,7 @@ from tests import helpers as H
 pytestmark = pytest.mark.gpu
 
 NAN = 0x7e00
+U32 = 2.0 ** -24
 SHAPES = [(32, 8, 128), (8, 1, 128), (4, 4, 128), (16, 4, 64), (3, 3, 64), (8, 2, 32), (2, 2, 32)]
 
 
@@ -359,3 +360,37 @@ def test_many_small_weights_count(gpu, heads, n, gap):
     c["vp"][:, :, ahead] = 0
     say("gap", gap, "of", n, heads)
     verify(run(gpu, c), closely(c))
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (8, 1, 128), (4, 4, 64), (8, 2, 32)])
+@pytest.mark.parametrize("prefix", [100, 3000])
+@pytest.mark.parametrize("scale", [300.0, 12000.0])
+def test_scores_of_any_magnitude(gpu, heads, prefix, scale):
+    """Queries and keys far up in their type's range (scores to 10^9 and more): the best position takes all the weight wherever it is
+    ahead by more than a score's error, (head_dim + 2) 2^-24 times the sum of |q k| (twice, for the two scores), and 40 (e^-40 of n
+    values of like size is far below half a step)."""
+    Hq, Hkv, hd = heads
+    c = case(33, 2, prefix, [0, 40], heads, False)
+    for name in ("qkv", "kp", "kcs"):
+        x = H.f16(c[name]) * scale
+        if name == "qkv":
+            x[:, (Hq + Hkv) * hd:] /= scale
+        c[name] = np.where(np.isnan(x), np.uint16(NAN), H.bits(np.clip(np.nan_to_num(x), -40000.0, 40000.0)))
+    got, kcs, vcs = run(gpu, c)
+    _, _, w_k, w_v = expected(c)
+    assert np.array_equal(kcs, w_k) and np.array_equal(vcs, w_v)
+    assert np.all(np.isfinite(H.f16(got)))
+    seen = 0
+    for z, pos in enumerate(c["positions"]):
+        q = H.f16(orc.rope(np.ascontiguousarray(c["qkv"][z:z + 1, :Hq * hd]), Hq, hd, pos)).reshape(Hq, hd)
+        for g in range(Hq):
+            h = g // (Hq // Hkv)
+            K = np.concatenate([H.f16(c["kp"][h, :prefix]), H.f16(w_k[z, h, prefix:pos + 1])])
+            V = np.concatenate([c["vp"][h, :, :prefix], w_v[z, h, :, prefix:pos + 1]], 1)
+            s, off = K @ q[g] / np.sqrt(hd), 2 * (hd + 2) * U32 * (np.abs(K) @ np.abs(q[g])).max() / np.sqrt(hd)
+            order = np.argsort(s)
+            if s[order[-1]] - s[order[-2]] > off + 40:
+                seen += 1
+                assert np.array_equal(got[z, g * hd:(g + 1) * hd], V[:, order[-1]]), (z, g)
+    say("rows with one position ahead:", seen, "of", 2 * Hq)
+    assert seen >= Hq
