@@ -227,11 +227,13 @@ long llama3_shared_prefix_steps(const CudaCache *c);
  * their log probabilities, largest first, the lowest id first among equals (id -1, -inf where fewer have a probability).  All
  * arrays are host memory, row after row.
  * llama3_logprobs: one row, the last one that c processed on its own (behind a batched step the call is refused: its rows are
- * with caches[0]).  llama3_batch_logprobs: every sequence of the last llama3_decode_batch with cache0 as caches[0].
+ * with caches[0]).  llama3_batch_logprobs: every sequence of the last llama3_decode_batch with cache0 as caches[0], whose number
+ * llama3_batch_rows returns (0: none has run): ids and the results hold that many rows.
  * llama3_score: llama3_prefill (appends the n tokens, returns the greedy next one) that also rates the text: logprob[i] is that
  * of tokens[i + 1] behind the tokens up to i (NaN for i = n - 1), entropy[i], top_ids/top_logprob[i * k ..] of the same row. */
 void llama3_logprobs(CudaCache *c, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k, int *top_ids,
                      float *top_logprob);
+int llama3_batch_rows(const CudaCache *cache0);
 void llama3_batch_logprobs(CudaCache *cache0, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
                            int *top_ids, float *top_logprob);
 int llama3_score(Llama3 *m, CudaCache *c, const int *tokens, int n, float temperature, float *logprob, float *entropy, int k,

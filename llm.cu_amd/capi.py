@@ -176,6 +176,7 @@ HOST_ABI = {
     "llama3_set_shared_prefix": (None, [_CP, _i]),
     "llama3_shared_prefix_steps": (C.c_long, [_CP]),
     "llama3_logprobs": (None, [_CP, C.c_float, _vp, _i, _vp, _vp, _i, _vp, _vp]),
+    "llama3_batch_rows": (_i, [_CP]),
     "llama3_batch_logprobs": (None, [_CP, C.c_float, _vp, _i, _vp, _vp, _i, _vp, _vp]),
     "llama3_score": (_i, [_LP, _CP, _vp, _i, C.c_float, _vp, _vp, _i, _vp, _vp]),
     "llama3_generate": (_i, [_LP, _CP, C.POINTER(_i), _i, _i, C.POINTER(_i), C.POINTER(GenStats)]),

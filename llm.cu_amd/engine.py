@@ -196,7 +196,8 @@ class Engine:
         return lib().llama3_shared_prefix_steps(self.cache)
 
     def _logprobs(self, fn, rows, ids, k, temperature):
-        ids = np.ascontiguousarray(ids, dtype=np.int32).reshape(rows, -1)
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        ids = ids.reshape(rows, ids.size // max(rows, 1))
         lp, ent = np.empty(ids.shape, np.float32), np.empty(rows, np.float32)
         ti, tl = np.empty((rows, k), np.int32), np.empty((rows, k), np.float32)
         fn(self.cache, temperature, ids.ctypes.data, ids.shape[1], lp.ctypes.data, ent.ctypes.data, k, ti.ctypes.data, tl.ctypes.data)
@@ -209,8 +210,15 @@ class Engine:
         return lp[0], float(ent[0]), ti[0], tl[0]
 
     def batch_logprobs(self, ids, k=0, temperature=1.0):
-        """The same for every sequence of the last decode_batch that began with this engine; ids [batch] or [batch, n]."""
-        return self._logprobs(lib().llama3_batch_logprobs, len(ids), ids, k, temperature)
+        """The same for every sequence of the last decode_batch that began with this engine; ids [batch] or [batch, n], or empty:
+        no given tokens."""
+        ids = np.asarray(ids, dtype=np.int32)
+        rows = lib().llama3_batch_rows(self.cache) or len(ids)  # no step yet: the library refuses the call
+        if ids.size == 0:
+            ids = ids.reshape(rows, 0)
+        if len(ids) != rows:  # the library reads and writes as many rows as the step had
+            raise ValueError("batch_logprobs: ids of %d sequences, the last batched step had %d" % (len(ids), rows))
+        return self._logprobs(lib().llama3_batch_logprobs, rows, ids, k, temperature)
 
     def score(self, tokens, k=0, temperature=1.0):
         """prefill that rates the text: (greedy next id, logprob [n] -- of tokens[i + 1] at i, NaN at the end --, entropy [n],

@@ -1010,6 +1010,8 @@ extern "C" void llama3_logprobs(CudaCache *C, float temperature, const int *ids,
     logprob_rows(e, e->logits, 1, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
 }
 
+extern "C" int llama3_batch_rows(const CudaCache *C0) { return eng(C0)->b_rows; }
+
 extern "C" void llama3_batch_logprobs(CudaCache *C0, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
                                       int *top_ids, float *top_logprob) {
     Engine *e = eng(C0);

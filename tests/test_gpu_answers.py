@@ -288,3 +288,27 @@ def test_refusals_end_with_a_message(gpu, code, text):
                         "m = pkg.engine.Model.seeded(cfg, 1).to_device(); a, b = pkg.engine.Engine(m, cfg), pkg.engine.Engine(m, cfg)\n" + code],
                        cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=120)
     assert p.returncode == 1 and text in p.stdout, p.stdout + p.stderr
+
+
+def test_batch_log_probabilities_take_one_row_per_sequence(tiny):
+    """Ids of more or of fewer sequences than the last batched step had are refused in front of the library's call, which reads and
+    writes as many rows as the step had; no ids at all are no given tokens."""
+    gpu, cfg, model = tiny
+    es = engines(gpu, cfg, model, 5)
+    es[0].prefill([1, 2, 3])
+    es[0].fork(es[1:])
+    gpu.engine.Engine.decode_batch(es, [4, 5, 6, 7, 8])
+    assert gpu.lib().llama3_batch_rows(es[0].cache) == 5 and gpu.lib().llama3_batch_rows(es[1].cache) == 0
+    for ids in ([7], [[7]], [1, 2, 3, 4], [1, 2, 3, 4, 5, 6], [[1, 2]] * 16):
+        with pytest.raises(ValueError, match="had 5"):
+            es[0].batch_logprobs(ids, 2)
+    for none in ([], [[], [], [], [], []]):
+        lp, ent, ti, tl = es[0].batch_logprobs(none, 2)
+        assert lp.shape == (5, 0) and ti.shape == (5, 2)
+        for z in range(5):
+            check_logprobs(es[0].batch_logits(z), 1.0, [], 2, (lp[z], ent[z], ti[z], tl[z]))
+    assert es[0].batch_logprobs([1, 2, 3, 4, 5])[0].shape == (5, 1)
+    gpu.engine.Engine.decode_batch(es[:2], [1, 2])
+    with pytest.raises(ValueError, match="had 2"):
+        es[0].batch_logprobs([1, 2, 3, 4, 5])
+    close_all(es)
