@@ -346,8 +346,8 @@ int llm_kv_fork(const uint16_t *k_src_dev, const uint16_t *v_src_dev, int src_ma
  * A logit of -inf is a token of probability 0: log probability -inf, never an alternative (id -1, -inf fill the places that
  * are left).  A row of -inf only: log probabilities -inf, entropy 0, no alternatives.  A row that holds a NaN or +inf has no
  * distribution: NaN in every float, -1 in every id.  Statistics are fp32, in an order that depends on the sizes only.
- * workspace: llm_logprobs_workspace_bytes, 16-byte aligned, zeroed once with llm_fill_zero before its first use (every call
- * leaves it reusable, by calls of other shapes too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured graphs.
+ * workspace: llm_logprobs_workspace_bytes, enough for every call of at most that many rows and alternatives, of any vocabulary;
+ * 16-byte aligned, zeroed once with llm_fill_zero before its first use (every call leaves it reusable); calls that share a workspace must not overlap, also not as nodes of two captured graphs.
  * No counterpart in the reference (its sampler keeps probabilities on the host, src/inference/inference.cu:1030-1061). */
 #define LLM_LOGPROBS_MAX_TOP 32
 #define LLM_LOGPROBS_MAX_IDS 16

@@ -33,6 +33,7 @@
 #define LP_MAX_CHUNKS 64       // of a row: one lane each when they are joined
 #define LP_MAX_VOCAB (1 << 20)
 #define LP_SLICE 4096          // rows per launch: a counter each at the front of the workspace
+#define LP_WORKGROUPS 512      // aimed at
 #define LP_LINE 32             // ints from one row's counter to the next: device-scope additions to one line wait for one another
 #define LP_LIST 768            // words of a wavefront's list: a row of 16-byte loads (512 logits) behind what it holds
 // Lanes above the bound up to which it stays, rather than being found anew.  With 0, 3, 8 and 16: 256 rows of 128256, 5 best, 26.5
@@ -411,7 +412,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
 }
 
 // How a row is cut.  Few rows: finely, so that their logits come from many compute units at once, but into LP_MAX_CHUNKS pieces
-// at most; many rows: coarsely, so that less is joined.  Aimed at 512 workgroups; with 256, 512 and 1024, rows of 128256: 64 rows,
+// at most; many rows: coarsely, so that less is joined.  Aimed at LP_WORKGROUPS; with 256, 512 and 1024, rows of 128256: 64 rows,
 // 20 best, 21.2 18.1 17.1 us, 256 rows, 5 best, 28.5 24.6 23.4, but 700 rows, 20 best, 54 54 69.
 // Short chunks in short segments, so that all wavefronts have one, long chunks in long ones with more loads in flight: with 1, 2
 // and 4 loads per lane 16 rows (chunks of 4096) 9.7 9.0 9.3 us, one row (2048) 8.4 and, with 4, 9.3, 2048 whole rows 110 with one
@@ -420,8 +421,7 @@ struct LpCut {
     int nl, chunk_len, chunks;
 };
 static LpCut lp_cut_row(int rows, int vocab) {
-    const int target = 512; // workgroups
-    int want = (target + rows - 1) / rows;
+    int want = (LP_WORKGROUPS + rows - 1) / rows;
     if (want > LP_MAX_CHUNKS) want = LP_MAX_CHUNKS;
     int len = (vocab + want - 1) / want;
     LpCut r = {};
@@ -439,10 +439,11 @@ template <int NL> static void lp_launch(const LpArgs &a, int rows, hipStream_t s
 
 extern "C" {
 
-// counters of LP_SLICE rows, then the statistics and lists of one launch
+// Counters of LP_SLICE rows, then the statistics and lists of one launch.  Fewer rows are cut into more chunks each, so this is a
+// bound for all calls of up to `rows` rows, whatever their vocabulary: rows * ceil(LP_WORKGROUPS / rows) < LP_WORKGROUPS + rows chunks.
 size_t llm_logprobs_workspace_bytes(int rows, int vocab, int k) {
     if (rows < 1 || vocab < 1 || vocab > LP_MAX_VOCAB || k < 0) return sizeof(int) * LP_SLICE * LP_LINE;
-    const size_t n = (size_t)(rows < LP_SLICE ? rows : LP_SLICE) * lp_cut_row(rows, vocab).chunks;
+    const size_t r = rows < LP_SLICE ? rows : LP_SLICE, most = r + LP_WORKGROUPS - 1, n = r * LP_MAX_CHUNKS < most ? r * LP_MAX_CHUNKS : most;
     return sizeof(int) * LP_SLICE * LP_LINE + n * (sizeof(uint32_t) * 4 + sizeof(lp_word) * k);
 }
 

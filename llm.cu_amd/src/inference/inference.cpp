@@ -592,12 +592,7 @@ int rows_in_common(Engine *const *es, int n) {
 
 void prepare_logprobs(Engine *e) {
     if (e->lp_ws) return;
-    size_t ws = 0;
-    for (int rows = 1; rows <= LP_ROWS; ++rows) {
-        const size_t need = llm_logprobs_workspace_bytes(rows, e->cfg.vocab, LLM_LOGPROBS_MAX_TOP);
-        ws = need > ws ? need : ws;
-    }
-    ws = (ws + 3) / 4 * 4;
+    const size_t ws = (llm_logprobs_workspace_bytes(LP_ROWS, e->cfg.vocab, LLM_LOGPROBS_MAX_TOP) + 3) / 4 * 4;
     e->lp_ids = dmalloc<int32_t>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_IDS, "llm_malloc(given tokens)");
     e->lp_out = dmalloc<float>((size_t)LP_ROWS * LLM_LOGPROBS_MAX_IDS, "llm_malloc(log probabilities)");
     e->lp_entropy = dmalloc<float>(LP_ROWS, "llm_malloc(entropies)");

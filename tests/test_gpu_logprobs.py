@@ -229,3 +229,19 @@ def test_captured_call(gpu):
             assert np.array_equal(got.download().view(np.uint32), want.view(np.uint32)), rep
     check(L.llm_graph_destroy(graph))
     check(L.llm_stream_destroy(stream))
+
+
+def test_a_workspace_for_many_rows_holds_a_call_of_fewer(gpu):
+    """511 rows are cut into two chunks each where 512 are not: the same workspace, and nothing is written behind it."""
+    vocab, k = 9000, 32
+    size = gpu.lib().llm_logprobs_workspace_bytes(512, vocab, k)
+    guard = 1 << 20
+    ws = gpu.capi.DevBuf((size + guard,), np.uint8)
+    mark = np.concatenate([np.zeros(size, np.uint8), np.full(guard, 0xa5, np.uint8)])
+    for rows in (512, 511, 256, 255, 8, 1):
+        x, ids = rows_of(rows, rows, vocab)
+        ws.upload(mark)
+        a = gpu.ops.logprobs(x, ids=ids, k=k, ws=ws)
+        assert np.all(ws.download()[size:] == 0xa5), rows
+        b = gpu.ops.logprobs(x, ids=ids, k=k)
+        assert all(np.array_equal(p.view(np.uint32), q.view(np.uint32)) for p, q in zip(a, b)), rows

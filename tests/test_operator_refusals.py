@@ -127,3 +127,23 @@ def test_logprobs(pkg, over, text):
 def test_logprobs_of_no_rows_and_of_no_tokens(pkg):
     assert logprobs(pkg) == pkg.capi.LLM_OK
     assert logprobs(pkg, n=0, ids=None, lp=None, k=0, ti=None, tl=None) == pkg.capi.LLM_OK
+
+
+def test_logprobs_workspace_holds_smaller_calls_too(pkg):
+    """The size never falls when rows or k grow, and is at least what a call of any smaller number of rows uses: counters for 4096
+    rows, 128 bytes each, then 16 bytes and k words of 8 for each chunk of a launch's rows; a row is cut into at most 64 chunks,
+    into no more than make 512 in all, rounded up to a chunk for each row."""
+    need = pkg.lib().llm_logprobs_workspace_bytes
+
+    def used(rows, k):
+        return 4096 * 128 + min(rows, 4096) * min(64, -(-512 // rows)) * (16 + 8 * k)
+
+    for vocab in (1, 64, 1000, 32003, 128256, 1 << 20):
+        for k in (0, 1, 5, 32):
+            last = 0
+            for rows in list(range(1, 700)) + [1023, 1024, 4095, 4096, 4097, 100000]:
+                size = need(rows, vocab, k)
+                assert size >= last and size == need(rows, 128256, k)
+                assert size >= used(rows, k) and (k == 0 or size > need(rows, vocab, k - 1))
+                last = size
+            assert need(600, vocab, k) >= max(used(r, k) for r in range(1, 601))
