@@ -12,9 +12,9 @@
 // rows, latency: 16 rows, 5 best 8.6 us, one row, 20 best 10.1 us, of which an empty launch through the same call is 7; on the
 // chip alone one row takes 5.0 us without alternatives, some 5 more with 20: the two levels of lists.
 //
-// Sums: exponentials are base 2, 2^(x c - R) with c = log2(e) / temperature and R = fl(m c) for the largest logit m so far: one
-// fused operation on the fp16 value, exact before its rounding.  A larger m rescales the lane's sums.  Parts are joined by their
-// R; what the rounding of m c shifted goes out again at the end.
+// Sums: exponentials are base 2, 2^((x - m) c) with c = log2(e) / temperature for the largest logit m so far.  The difference comes
+// first: it is exact or rounded once, so the largest logit has weight 1 at any temperature (a fused x c - m c is off by the rounding
+// of m c, which passes the range of 2^y at m / temperature = 4e9).  A larger m rescales the lane's sums.
 //
 // The k best (k <= 32) without a sort: the k-th largest of a wavefront's 64 running lane maxima is a lower bound of its k-th
 // largest logit, found digit by digit on 16-bit order keys (ballots and bit counts, two bits a step).  The few logits from there up are
@@ -59,7 +59,7 @@ struct LpArgs {
 };
 
 struct LpStats {
-    float m, s, t; // largest logit, sum of 2^y, sum of y 2^y with y = x c - fl(m c)
+    float m, s, t; // largest logit, sum of 2^(d c), sum of d 2^(d c) with d = x - m
 };
 
 __device__ __forceinline__ void lp_put(uint32_t *p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -81,11 +81,11 @@ __device__ __forceinline__ half_t lp_value(uint32_t key) { // the logit of an or
 __device__ __forceinline__ lp_word lp_make(half_t h, int index) { return (lp_word)lp_key(h) << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t lp_word_key(lp_word w) { return (uint32_t)(w >> 32); }
 
-__device__ __forceinline__ float lp_ref(float m, float c) { return m == -INFINITY ? 0.f : m * c; }
+__device__ __forceinline__ float lp_base(float m) { return m == -INFINITY ? 0.f : m; }
 
 // sums relative to the reference of a larger maximum M
 __device__ __forceinline__ LpStats lp_rebase(LpStats p, float M, float c) {
-    const float d = lp_ref(p.m, c) - lp_ref(M, c), f = p.s == 0.f ? 0.f : __builtin_amdgcn_exp2f(d);
+    const float d = lp_base(p.m) - lp_base(M), f = p.s == 0.f ? 0.f : __builtin_amdgcn_exp2f(d * c);
     return {M, f * p.s, f == 0.f ? 0.f : f * (p.t + d * p.s)};
 }
 
@@ -233,6 +233,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     const size_t row = blockIdx.y;
     const half_t *x = a.x + row * a.ld;
     const float c = a.inv_t * 1.44269504088896341f;
+    float one = 1.f;
+    asm("" : "+v"(one)); // not folded: a multiplication, so that conversion and difference are one instruction
     const half_t ninf = __builtin_bit_cast(half_t, (uint16_t)0xfc00u);
     lp_word *list = lists + wave * LP_LIST;
 
@@ -280,14 +282,14 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
             top = lane_max[u] > top ? lane_max[u] : top;
         }
         if (__builtin_amdgcn_ballot_w64((float)top > st.m)) st = lp_rebase(st, fmaxf(st.m, wave_max((float)top)), c);
-        const float ref = lp_ref(st.m, c);
+        const float base = lp_base(st.m);
 #pragma unroll
         for (int u = 0; u < NL; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = fmaf((float)v[u][e], c, -ref), p = __builtin_amdgcn_exp2f(y);
+                const float d = fmaf((float)v[u][e], one, -base), p = __builtin_amdgcn_exp2f(d * c);
                 st.s += p;
-                st.t = fmaf(fmaxf(y, -FLT_MAX), p, st.t); // -inf times zero is zero here; a NaN is in p already
+                st.t = fmaf(fmaxf(d, -FLT_MAX), p, st.t); // -inf times zero is zero here; a NaN is in p already
             }
         lane_best = top > lane_best ? top : lane_best;
         const int lanes = k > 0 ? __popcll(__builtin_amdgcn_ballot_w64(top >= from)) : 0;
@@ -395,9 +397,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     }
     // ---- 4. results ------------------------------------------------------------------------------------------------------
     const bool invalid = st.s != st.s, none = st.s == 0.f;
-    const float m0 = none ? 0.f : st.m, off = fmaf(m0, c, -lp_ref(m0, c)); // sums stand at 2^off times their value for m c itself
-    const float mean = none ? 0.f : (st.t / st.s - off) * 0.693147180559945309f;
-    const float log_s = none ? 0.f : logf(st.s) - off * 0.693147180559945309f;
+    const float m0 = none ? 0.f : st.m, mean = none ? 0.f : st.t / st.s * a.inv_t, log_s = none ? 0.f : logf(st.s);
     if (tid == 0) a.entropy[row] = invalid ? NAN : log_s - mean;
     if (tid < a.n_ids) {
         float lp = NAN;

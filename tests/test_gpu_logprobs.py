@@ -245,3 +245,23 @@ def test_a_workspace_for_many_rows_holds_a_call_of_fewer(gpu):
         assert np.all(ws.download()[size:] == 0xa5), rows
         b = gpu.ops.logprobs(x, ids=ids, k=k)
         assert all(np.array_equal(p.view(np.uint32), q.view(np.uint32)) for p, q in zip(a, b)), rows
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-20, 1e-12, 1e-10, 1e-9, 1e-8, 1e-6, 1e-5, 1e-3, 1e-2, 1e4, 1e30, 3.4e38])
+@pytest.mark.parametrize("vocab", [2, 1003, 70001])
+def test_temperatures_over_the_accepted_range(gpu, temperature, vocab):
+    """Maxima whose products with the reciprocal temperature are rounded, from the smallest logits to the largest; rows with two
+    equal maxima, with a mask, and of one magnitude throughout."""
+    peaks = [6.30, 12.5, 13.25, 14.3, 39.9, 65504.0, -65504.0, 6e-8, 0.333, -7.77]
+    x, _ = rows_of(17, 2 * len(peaks), vocab)
+    ids = np.zeros((2 * len(peaks), 2), np.int32)
+    for r, peak in enumerate(peaks):
+        for row in (r, r + len(peaks)):
+            top = H.bits(peak).item()
+            x[row] = H.bits(np.maximum(np.minimum(H.f16(x[row]), peak - abs(peak) * 2.0 ** -9), -65504.0))
+            x[row, vocab // 3] = top
+            ids[row] = vocab // 3, vocab - 1
+        x[r + len(peaks), vocab - 1] = top   # the second of two equal ones
+        x[r, : vocab // 4] = NINF
+    say("temperature", temperature, "vocab", vocab)
+    verify(gpu, x, ids=ids, k=min(vocab, 5), temperature=temperature)
