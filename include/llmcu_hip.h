@@ -338,7 +338,7 @@ int llm_kv_fork(const uint16_t *k_src_dev, const uint16_t *v_src_dev, int src_ma
                 int head_dim, llm_stream_t stream);
 
 /* ---- log probabilities ---------------------------------------------------------------------------------- */
-/* For every row of fp16 logits ([rows, ld], vocab columns used, at most 1048576; rows may start at any element): with y = logit / temperature (1e-30 or more),
+/* For every row of fp16 logits ([rows, ld], at most 2^31 - 4097 rows; vocab columns used, at most 1048576; rows may start at any element): with y = logit / temperature (1e-30 or more),
  *   logprob_dev[row][i] = y[ids[row][i]] - logsumexp(y)   for n_ids (0..16) given tokens, NaN for an id outside [0, vocab)
  *   entropy_dev[row]    = -sum p ln p,  p = softmax(y)
  *   top_ids_dev[row][j], top_logprob_dev[row][j]: the k (0..32, at most vocab) tokens of largest logit and their log

@@ -22,6 +22,7 @@
 // best, after which only larger logits can enter, since equal ones further back lose.  A listed logit is a 64-bit word, order
 // key above the complement of its index.
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 #include "common.hpp"
@@ -450,6 +451,7 @@ size_t llm_logprobs_workspace_bytes(int rows, int vocab, int k) {
 int llm_logprobs(const uint16_t *logits, int ld, int rows, int vocab, float temperature, const int32_t *ids, int n_ids,
                  float *logprob, float *entropy, int k, int32_t *top_ids, float *top_logprob, void *workspace, llm_stream_t stream) {
     LLM_REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab, "llm_logprobs: %d rows of %d logits, ld=%d", rows, vocab, ld);
+    LLM_REQUIRE(rows <= INT_MAX - LP_SLICE, "llm_logprobs: %d rows (at most %d)", rows, INT_MAX - LP_SLICE);
     LLM_REQUIRE(vocab <= LP_MAX_VOCAB, "llm_logprobs: %d logits per row (at most %d)", vocab, LP_MAX_VOCAB);
     LLM_REQUIRE(temperature >= 1e-30f && temperature <= FLT_MAX, "llm_logprobs: temperature %g (at least 1e-30)", (double)temperature);
     LLM_REQUIRE(n_ids >= 0 && n_ids <= LP_MAX_IDS, "llm_logprobs: %d given tokens per row (0..%d)", n_ids, LP_MAX_IDS);

@@ -147,3 +147,9 @@ def test_logprobs_workspace_holds_smaller_calls_too(pkg):
                 assert size >= used(rows, k) and (k == 0 or size > need(rows, vocab, k - 1))
                 last = size
             assert need(600, vocab, k) >= max(used(r, k) for r in range(1, 601))
+
+
+@pytest.mark.parametrize("rows", [2 ** 31 - 1, 2 ** 31 - 512, 2 ** 31 - 4096])
+def test_logprobs_of_more_rows_than_can_be_counted(pkg, rows):
+    """Next to the type's end the cut of a row divided by zero and the loop over slices ran past it."""
+    refused(pkg, logprobs(pkg, rows=rows, vocab=1, ld=1, k=1), "at most")
