@@ -399,7 +399,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
     // ---- 4. results ------------------------------------------------------------------------------------------------------
     const bool invalid = st.s != st.s, none = st.s == 0.f;
     const float m0 = none ? 0.f : st.m, mean = none ? 0.f : st.t / st.s * a.inv_t, log_s = none ? 0.f : logf(st.s);
-    if (tid == 0) a.entropy[row] = invalid ? NAN : log_s - mean;
+    if (tid == 0) a.entropy[row] = invalid ? NAN : fmaxf(log_s - mean, 0.f); // where it is about 0, roundings may have either sign
     if (tid < a.n_ids) {
         float lp = NAN;
         if (id >= 0 && id < a.vocab && !invalid) lp = ((float)given - m0) * a.inv_t - log_s;

@@ -265,3 +265,16 @@ def test_temperatures_over_the_accepted_range(gpu, temperature, vocab):
         x[r, : vocab // 4] = NINF
     say("temperature", temperature, "vocab", vocab)
     verify(gpu, x, ids=ids, k=min(vocab, 5), temperature=temperature)
+
+
+def test_entropy_is_never_negative(gpu):
+    """Rows with one logit ahead by anything from nothing to all: ln S and the mean that is taken from it are rounded apart."""
+    for vocab in (2, 50, 5000):
+        rng = np.random.default_rng(vocab)
+        x = H.bits(rng.standard_normal((400, vocab)))
+        x[:, 0] = H.bits(np.linspace(3, 40, 400))
+        for t in (1e-8, 1e-3, 0.3, 1.0, 2.0):
+            _, ent, _, _ = gpu.ops.logprobs(x, temperature=t)
+            say("vocab", vocab, "temperature", t, "least", ent.min())
+            assert ent.min() >= 0.0
+        verify(gpu, x[::40])

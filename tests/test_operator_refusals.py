@@ -151,5 +151,5 @@ def test_logprobs_workspace_holds_smaller_calls_too(pkg):
 
 @pytest.mark.parametrize("rows", [2 ** 31 - 1, 2 ** 31 - 512, 2 ** 31 - 4096])
 def test_logprobs_of_more_rows_than_can_be_counted(pkg, rows):
-    """Next to the type's end the cut of a row divided by zero and the loop over slices ran past it."""
+    """Next to the type's end the cut of a row and the loop over slices would overflow it."""
     refused(pkg, logprobs(pkg, rows=rows, vocab=1, ld=1, k=1), "at most")
