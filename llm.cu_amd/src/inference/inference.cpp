@@ -573,7 +573,8 @@ void issue_batch_step(Engine *e0, const Llama3 *m, int batch, int form) {
 
 bool same_config(const ModelConfig &a, const ModelConfig &b) {
     return a.max_pos == b.max_pos && a.d_model == b.d_model && a.n_layers == b.n_layers && a.vocab == b.vocab &&
-           a.n_heads == b.n_heads && a.n_kv_heads == b.n_kv_heads && a.head_dim == b.head_dim;
+           a.n_heads == b.n_heads && a.n_kv_heads == b.n_kv_heads && a.head_dim == b.head_dim && a.ffn_dim == b.ffn_dim &&
+           a.rms_eps == b.rms_eps && a.rope_theta == b.rope_theta; // cached keys hold their rotation
 }
 
 // Rows that all of the caches hold bit for bit.

@@ -312,3 +312,11 @@ def test_batch_log_probabilities_take_one_row_per_sequence(tiny):
     with pytest.raises(ValueError, match="had 2"):
         es[0].batch_logprobs([1, 2, 3, 4, 5])
     close_all(es)
+
+
+@pytest.mark.parametrize("over", ["rope_theta=10000.0", "rms_eps=1e-6"])
+@pytest.mark.parametrize("call", ["a.fork([c])", "a.fork([b, c])", "E.decode_batch([a, c], [1, 2])", "E.decode_batch([c, b], [1, 2])"])
+def test_caches_that_rotate_or_normalise_otherwise_are_refused(gpu, over, call):
+    """Their rows, and the (cos, sin) table that a batched step takes from its first cache, would not fit together."""
+    test_refusals_end_with_a_message(gpu, "E = pkg.engine.Engine; c = E(m, pkg.engine.config('tiny', %s)); a.prefill([1]); %s" % (over, call),
+                                     "different configuration")
