@@ -211,9 +211,10 @@ void llama3_read_batch_logits(CudaCache *cache0, int b, llm_half *logits);
 
 /* Several answers to one prompt.
  * llama3_fork: dsts[0..n-1] (1..16 caches of the same configuration) become copies of src: its cached rows, ids, position and
- * the logits of the last row that it processed on its own.  Each stands for itself afterwards and takes every call of this interface; what it held before is gone.  Rows
- * that a destination has in common with src from an earlier fork are not copied again, so an answer that branches from its
- * sibling costs its own tokens only.
+ * the logits of the last row that it processed on its own.  Each stands for itself afterwards and takes every call of this
+ * interface, with the model that src was last used with (another one is refused until llama3_cache_reset); what it held before is
+ * gone.  Rows that a destination has in common with src from an earlier fork are not copied again, so an answer that branches
+ * from its sibling costs its own tokens only.
  * llama3_decode_batch on caches that have rows in common reads those rows once for all sequences
  * (llm_attn_decode_rope_shared_dev) where that is faster: 512 rows or more, and 4096 or more times the batch.  The sums of the
  * attention run in another order then.  llama3_set_shared_prefix(caches[0], mode): 0 never, 1 (default) as said, 2 with any row

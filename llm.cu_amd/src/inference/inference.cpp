@@ -106,6 +106,9 @@ struct Engine {
         int len;
     };
     std::vector<SharedRows> marks;
+    // the model that computed the rows which llama3_fork brought (null: no fork brought any)
+    const Llama3 *fork_model = nullptr;
+    const void *fork_slab = nullptr;
     int shared_mode = 1;    // 0: batched steps never read a shared prefix once for all, 1: where it is faster, 2: always
     long shared_steps = 0;  // batched steps with this cache as sequence 0 that did
     llm_shared_desc *b_shared = nullptr, *b_shared_host = nullptr;
@@ -205,8 +208,17 @@ void drop_graph(Engine *e) {
 // The captured decode graphs hold the weight pointers of the model they were captured with.  A call
 // with another model (or the same struct after its weights were reloaded) is checked against the
 // configuration like the first one and the graphs are captured again.
+const void *model_slab(const Llama3 *m) { return m && m->embed_tokens ? (const void *)m->embed_tokens->d_fp16_tensor : nullptr; }
+
+// Rows that a fork brought continue under the model that computed them.
+void check_fork_model(const Engine *e, const Llama3 *m) {
+    if (e->pos > 0 && e->fork_model && (m != e->fork_model || model_slab(m) != e->fork_slab))
+        llama3_fail("the cache's rows were forked from a cache of another model");
+}
+
 void bind_model(Engine *e, const Llama3 *m) {
-    const void *slab = m && m->embed_tokens ? (const void *)m->embed_tokens->d_fp16_tensor : nullptr;
+    check_fork_model(e, m);
+    const void *slab = model_slab(m);
     if (m == e->model && slab == e->model_slab) return;
     check_shapes(m, e->cfg);
     drop_graph(e);
@@ -767,6 +779,8 @@ extern "C" void llama3_cache_reset(CudaCache *C) {
     e->logits_pos = 0;
     e->tokens.clear();
     e->marks.clear();
+    e->fork_model = nullptr;
+    e->fork_slab = nullptr;
     e->dev_pos_valid = false;
     e->dev_next = -1;
 }
@@ -859,6 +873,7 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
             if (es[a] == es[b]) llama3_fail("llama3_decode_batch: sequence %d and %d share a cache", a, b);
         if (!same_config(es[b]->cfg, c))
             llama3_fail("llama3_decode_batch: cache %d has a different configuration", b);
+        check_fork_model(es[b], m);
         if (es[b]->pos + 1 > c.max_pos) llama3_fail("sequence of %d tokens exceeds max_pos %d", es[b]->pos + 1, c.max_pos);
         if (tokens[b] < 0 || tokens[b] >= c.vocab) llama3_fail("token id %d outside the vocabulary", tokens[b]);
         pos[b] = es[b]->pos;
@@ -984,6 +999,8 @@ extern "C" void llama3_fork(CudaCache *src, CudaCache *const *dsts, int n) {
         es[i]->pos = e->pos;
         es[i]->logits_pos = e->logits_pos;
         es[i]->marks = e->marks;
+        es[i]->fork_model = e->fork_model ? e->fork_model : e->model;
+        es[i]->fork_slab = e->fork_model ? e->fork_slab : e->model_slab;
         es[i]->dev_pos_valid = false; // its device copies of position and ids are those of what it held before
         es[i]->dev_next = -1;
     }

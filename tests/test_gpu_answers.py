@@ -320,3 +320,30 @@ def test_caches_that_rotate_or_normalise_otherwise_are_refused(gpu, over, call):
     """Their rows, and the (cos, sin) table that a batched step takes from its first cache, would not fit together."""
     test_refusals_end_with_a_message(gpu, "E = pkg.engine.Engine; c = E(m, pkg.engine.config('tiny', %s)); a.prefill([1]); %s" % (over, call),
                                      "different configuration")
+
+
+OTHER = "E = pkg.engine.Engine; n = pkg.engine.Model.seeded(cfg, 2).to_device(); c = E(n, cfg); a.prefill([1, 2]); a.fork([c]); "
+
+
+@pytest.mark.parametrize("call", ["c.decode(3)", "c.prefill([3])", "c.generate([3], 2)", "c.score([3])", "E.decode_batch([c, b], [1, 2])",
+                                  "E.decode_batch([a, c], [1, 2]); print('taken'); c.decode(3)", "c.fork([b]); b.fork([c]); c.decode(3)"])
+def test_forked_rows_do_not_continue_under_another_model(gpu, call):
+    """A fork into an engine of other weights holds rows that those did not compute; steps of the source's model take it."""
+    test_refusals_end_with_a_message(gpu, OTHER + call, "another model")
+
+
+def test_a_reset_fork_takes_any_model(tiny):
+    gpu, cfg, model = tiny
+    other = gpu.engine.Model.seeded(cfg, 5).to_device()
+    a, b, c = engines(gpu, cfg, model, 1) + engines(gpu, cfg, other, 2)
+    a.prefill([1, 2, 3])
+    a.fork([b])
+    b.reset()
+    assert b.prefill([4, 5])[0] == c.prefill([4, 5])[0] and np.array_equal(b.logits(), c.logits())
+    c.fork([a])
+    a.reset()
+    a.prefill([1, 2, 3])
+    c.fork([b])
+    assert b.decode(6)[0] == c.decode(6)[0]
+    close_all([a, b, c])
+    other.close()
