@@ -97,7 +97,7 @@ struct Engine {
     int32_t *b_ids_host = nullptr;
     llm_graph_t b_graph[17][2] = {};
     bool b_ran[17][2] = {};
-    int b_rows = 0; // sequences of the last batched step (rows of b_logits)
+    int b_rows = 0; // sequences of the last batched step since a reset (rows of b_logits)
     int logits_pos = 0; // tokens behind the last of which `logits` stands (batched steps leave theirs in b_logits)
     // Rows that other caches hold bit for bit, from llama3_fork: caches with a mark of the same id agree on rows 0 .. len - 1.
     // Marks grow in len; only llama3_cache_reset takes rows back, and with them the marks.
@@ -777,6 +777,7 @@ extern "C" void llama3_cache_reset(CudaCache *C) {
     Engine *e = eng(C);
     e->pos = 0;
     e->logits_pos = 0;
+    e->b_rows = 0;
     e->tokens.clear();
     e->marks.clear();
     e->fork_model = nullptr;

@@ -347,3 +347,8 @@ def test_a_reset_fork_takes_any_model(tiny):
     assert b.decode(6)[0] == c.decode(6)[0]
     close_all([a, b, c])
     other.close()
+
+
+def test_batch_log_probabilities_are_gone_with_a_reset(gpu):
+    test_refusals_end_with_a_message(gpu, BATCHED + "print(a.batch_logprobs([1, 2])[0].shape); a.reset(); "
+                                     "assert pkg.lib().llama3_batch_rows(a.cache) == 0; a.prefill([1]); a.batch_logprobs([1, 2])", "no batch step")
