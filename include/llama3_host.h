@@ -231,7 +231,9 @@ long llama3_shared_prefix_steps(const CudaCache *c);
  * with caches[0]).  llama3_batch_logprobs: every sequence of the last llama3_decode_batch with cache0 as caches[0], whose number
  * llama3_batch_rows returns (0: none since cache0 was created or reset): ids and the results hold that many rows.
  * llama3_score: llama3_prefill (appends the n tokens, returns the greedy next one) that also rates the text: logprob[i] is that
- * of tokens[i + 1] behind the tokens up to i (NaN for i = n - 1), entropy[i], top_ids/top_logprob[i * k ..] of the same row. */
+ * of tokens[i + 1] behind the tokens up to i (NaN for i = n - 1), entropy[i], top_ids/top_logprob[i * k ..] of the same row.
+ * The last row is that of llama3_logprobs, bit for bit (its best alternative is the returned id); the rows in front of it come from
+ * one product, which rounds otherwise than single steps. */
 void llama3_logprobs(CudaCache *c, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k, int *top_ids,
                      float *top_logprob);
 int llama3_batch_rows(const CudaCache *cache0);

@@ -1041,18 +1041,20 @@ extern "C" int llama3_score(Llama3 *m, CudaCache *C, const int *tokens, int n, f
     check_logprob_args(e, 1, k, tokens, logprob, top_ids, top_logprob);
     const int next = run_pass(e, m, tokens, n); // leaves the residual stream of its rows in e->x
     llm_stream_t s = e->stream;
-    const int d = c.d_model, at_once = n < LP_ROWS ? n : LP_ROWS;
-    if (!e->score_logits) e->score_logits = dmalloc<llm_half>((size_t)(c.max_pos < LP_ROWS ? c.max_pos : LP_ROWS) * c.vocab, "llm_malloc(logits of a scored pass)");
-    llama3_check(llm_rmsnorm(e->x, m->norm->d_fp16_tensor, e->xn, n, d, c.rms_eps, s), "llm_rmsnorm");
-    std::vector<int> given((size_t)n);
-    for (int i = 0; i < n; ++i) given[i] = i + 1 < n ? tokens[i + 1] : -1; // no token is known behind the last one
-    for (int r0 = 0; r0 < n; r0 += at_once) {
-        const int rows = n - r0 < at_once ? n - r0 : at_once;
+    // the last row from the logits that the returned id was picked from: a product over many rows rounds otherwise
+    const int d = c.d_model, last = n - 1, at_once = last < LP_ROWS ? last : LP_ROWS;
+    if (last > 0 && !e->score_logits) e->score_logits = dmalloc<llm_half>((size_t)(c.max_pos < LP_ROWS ? c.max_pos : LP_ROWS) * c.vocab, "llm_malloc(logits of a scored pass)");
+    if (last > 0) llama3_check(llm_rmsnorm(e->x, m->norm->d_fp16_tensor, e->xn, last, d, c.rms_eps, s), "llm_rmsnorm");
+    for (int r0 = 0; r0 < last; r0 += at_once) {
+        const int rows = last - r0 < at_once ? last - r0 : at_once;
         llama3_check(llm_linear(e->xn + (size_t)r0 * d, d, m->lm_head->d_fp16_tensor, nullptr, 0, e->score_logits, c.vocab, rows, c.vocab, d, s),
                      "llm_linear(lm_head)");
-        logprob_rows(e, e->score_logits, rows, temperature, given.data() + r0, 1, logprob + r0, entropy ? entropy + r0 : nullptr, k,
+        logprob_rows(e, e->score_logits, rows, temperature, tokens + r0 + 1, 1, logprob + r0, entropy ? entropy + r0 : nullptr, k,
                      top_ids ? top_ids + (size_t)r0 * k : nullptr, top_logprob ? top_logprob + (size_t)r0 * k : nullptr);
     }
+    const int none = -1; // no token is known behind the last one
+    logprob_rows(e, e->logits, 1, temperature, &none, 1, logprob + last, entropy ? entropy + last : nullptr, k,
+                 top_ids ? top_ids + (size_t)last * k : nullptr, top_logprob ? top_logprob + (size_t)last * k : nullptr);
     return next;
 }
 

@@ -352,3 +352,19 @@ def test_a_reset_fork_takes_any_model(tiny):
 def test_batch_log_probabilities_are_gone_with_a_reset(gpu):
     test_refusals_end_with_a_message(gpu, BATCHED + "print(a.batch_logprobs([1, 2])[0].shape); a.reset(); "
                                      "assert pkg.lib().llama3_batch_rows(a.cache) == 0; a.prefill([1]); a.batch_logprobs([1, 2])", "no batch step")
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 33, 513, 514, 700])
+def test_the_last_row_of_a_score_is_that_of_the_returned_id(tiny, n):
+    gpu, cfg, model = tiny
+    a = engines(gpu, cfg, model, 1)[0]
+    for seed in range(4):
+        a.reset()
+        for t in (1.0, 0.4):
+            nxt, lp, ent, ti, tl = a.score([int(x) for x in gpu.engine.seeded_tokens(seed + 1, n, cfg.vocab)], k=7, temperature=t)
+            _, e, i, l = a.logprobs(k=7, temperature=t)
+            assert ti[-1][0] == nxt and np.isnan(lp[-1])
+            assert np.float32(e) == ent[-1] and np.array_equal(i, ti[-1]) and np.array_equal(l.view(np.uint32), tl[-1].view(np.uint32))
+            if n > 511:
+                a.reset()
+    a.close()
