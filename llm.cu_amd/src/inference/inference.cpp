@@ -14,6 +14,7 @@
 //   copy + O projection, add  -> llm_linear with the residual in its epilogue
 //   gate/up+SiLU, down, add   -> llm_linear_swiglu, llm_linear with residual
 #include <atomic>
+#include <cfloat>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -615,7 +616,8 @@ void prepare_logprobs(Engine *e) {
     llama3_check(llm_fill_zero(e->lp_ws, ws, e->stream), "zero log probability workspace");
 }
 
-void check_logprob_args(const Engine *e, int n_ids, int k, const void *ids, const void *logprob, const void *top_ids, const void *top) {
+void check_logprob_args(const Engine *e, float temperature, int n_ids, int k, const void *ids, const void *logprob, const void *top_ids, const void *top) {
+    if (!(temperature >= 1e-30f && temperature <= FLT_MAX)) llama3_fail("log probabilities: temperature %g (at least 1e-30)", (double)temperature);
     if (n_ids < 0 || n_ids > LLM_LOGPROBS_MAX_IDS) llama3_fail("log probabilities of %d given tokens (0..%d)", n_ids, LLM_LOGPROBS_MAX_IDS);
     if (k < 0 || k > LLM_LOGPROBS_MAX_TOP || k > e->cfg.vocab) llama3_fail("top %d alternatives (0..%d, at most the vocabulary)", k, LLM_LOGPROBS_MAX_TOP);
     if ((n_ids > 0 && (!ids || !logprob)) || (k > 0 && (!top_ids || !top))) llama3_fail("log probabilities: null pointer");
@@ -1018,7 +1020,7 @@ extern "C" long llama3_shared_prefix_steps(const CudaCache *C) { return eng(C)->
 extern "C" void llama3_logprobs(CudaCache *C, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
                                 int *top_ids, float *top_logprob) {
     Engine *e = eng(C);
-    check_logprob_args(e, n_ids, k, ids, logprob, top_ids, top_logprob);
+    check_logprob_args(e, temperature, n_ids, k, ids, logprob, top_ids, top_logprob);
     if (e->pos == 0) llama3_fail("llama3_logprobs: no row has been processed");
     if (e->logits_pos != e->pos) llama3_fail("llama3_logprobs: the last row was a batched step's (llama3_batch_logprobs)");
     logprob_rows(e, e->logits, 1, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
@@ -1029,7 +1031,7 @@ extern "C" int llama3_batch_rows(const CudaCache *C0) { return eng(C0)->b_rows; 
 extern "C" void llama3_batch_logprobs(CudaCache *C0, float temperature, const int *ids, int n_ids, float *logprob, float *entropy, int k,
                                       int *top_ids, float *top_logprob) {
     Engine *e = eng(C0);
-    check_logprob_args(e, n_ids, k, ids, logprob, top_ids, top_logprob);
+    check_logprob_args(e, temperature, n_ids, k, ids, logprob, top_ids, top_logprob);
     if (e->b_rows == 0) llama3_fail("llama3_batch_logprobs: no batch step has run");
     logprob_rows(e, e->b_logits, e->b_rows, temperature, ids, n_ids, logprob, entropy, k, top_ids, top_logprob);
 }
@@ -1038,7 +1040,7 @@ extern "C" int llama3_score(Llama3 *m, CudaCache *C, const int *tokens, int n, f
                             int *top_ids, float *top_logprob) {
     Engine *e = eng(C);
     const ModelConfig &c = e->cfg;
-    check_logprob_args(e, 1, k, tokens, logprob, top_ids, top_logprob);
+    check_logprob_args(e, temperature, 1, k, tokens, logprob, top_ids, top_logprob);
     const int next = run_pass(e, m, tokens, n); // leaves the residual stream of its rows in e->x
     llm_stream_t s = e->stream;
     // the last row from the logits that the returned id was picked from: a product over many rows rounds otherwise

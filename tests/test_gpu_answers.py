@@ -368,3 +368,10 @@ def test_the_last_row_of_a_score_is_that_of_the_returned_id(tiny, n):
             if n > 511:
                 a.reset()
     a.close()
+
+
+@pytest.mark.parametrize("temperature", ["0.0", "-1.0", "float('nan')", "float('inf')"])
+def test_a_refused_score_appends_nothing(gpu, temperature):
+    """The temperature is looked at in front of the pass, like the other arguments."""
+    test_refusals_end_with_a_message(gpu, "import ctypes; cb = ctypes.CFUNCTYPE(None, ctypes.c_char_p)(lambda s: print('refused at', a.pos, s, flush=True))\n"
+                                     "pkg.lib().llama3_set_error_handler(cb); a.prefill([1]); a.score([2, 3], 1, %s)" % temperature, "refused at 1 ")
