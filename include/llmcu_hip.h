@@ -278,7 +278,7 @@ int llm_attn_decode_rope_batch_dev(const uint16_t *qkv_dev, int ldq, const llm_b
  * Row r of every own cache ([n_kv_heads][max_pos][head_dim]) holds position row0 + r, 0 <= row0 <= prefix_len: 0 for caches
  * that hold the prefix too (their rows below prefix_len are not read), prefix_len for caches that hold the answers only.
  * positions[z] < row0 + max_pos; table_dev covers row0 + max_pos positions.  The prefix cache may be one of the own caches
- * (with row0 = 0 and prefix_max_pos = max_pos); own caches are distinct.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
+ * (with row0 = 0 and prefix_max_pos = max_pos); own caches have no memory in common, with one another or otherwise with the prefix.  max_pos and prefix_max_pos are multiples of 64, one head's keys stay below
  * 2 GiB.  Rows that hold no position yet may hold anything, NaN included.
  * Arithmetic: queries and the new key are rounded to fp16 after the rotation (llm_rope's results), products on the matrix
  * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32; a softmax weight is the sum of two fp16

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "ranges.hpp"
 
 struct SharedArgs {
     const half_t *qkv;
@@ -814,16 +815,24 @@ int llm_attn_decode_rope_shared(const uint16_t *qkv, int ldq, const uint16_t *k_
     a.host.v_prefix = v_prefix;
     a.host.prefix_len = prefix_len;
     a.host.row0 = row0;
+    // Memory in common would make the appended rows race with what is read: none between the own caches, and with the prefix only
+    // all of it, both halves, where the new rows lie behind the prefix.
+    const size_t per_row = sizeof(half_t) * (size_t)n_kv_heads * head_dim, own_bytes = per_row * max_pos;
+    const size_t prefix_bytes = prefix_len > 0 ? per_row * prefix_max_pos : 0;
     for (int z = 0; z < batch; ++z) {
         LLM_REQUIRE(k_caches[z] && v_caches[z] && aligned16(k_caches[z]) && aligned16(v_caches[z]), "%s: cache %d", name, z);
         LLM_REQUIRE(positions[z] >= prefix_len && (long long)positions[z] - row0 < max_pos, "%s: position %d (the prefix has %d, the caches hold %d..%lld)",
                     name, positions[z], prefix_len, row0, (long long)row0 + max_pos - 1);
+        auto meets = [&](const void *half, size_t bytes) {
+            return bytes > 0 && (ranges_meet(half, bytes, k_caches[z], own_bytes) || ranges_meet(half, bytes, v_caches[z], own_bytes));
+        };
         // a prefix inside one of the own caches stays where it is only if row r of that cache is position r
-        LLM_REQUIRE(prefix_len == 0 || (k_caches[z] != k_prefix && v_caches[z] != v_prefix) ||
-                        (k_caches[z] == k_prefix && v_caches[z] == v_prefix && row0 == 0 && prefix_max_pos == max_pos),
-                    "%s: the prefix lies in cache %d, whose row 0 is not position 0 or whose size is another", name, z);
+        const bool in_place = k_caches[z] == k_prefix && v_caches[z] == v_prefix && row0 == 0 && prefix_max_pos == max_pos;
+        LLM_REQUIRE(in_place || !(meets(k_prefix, prefix_bytes) || meets(v_prefix, prefix_bytes)),
+                    "%s: the prefix lies in cache %d, whose row 0 is not position 0, whose size is another or of which it is only a part", name, z);
+        LLM_REQUIRE(!ranges_meet(k_caches[z], own_bytes, v_caches[z], own_bytes), "%s: the halves of cache %d overlap", name, z);
         for (int y = 0; y < z; ++y)
-            LLM_REQUIRE(k_caches[y] != k_caches[z] && v_caches[y] != v_caches[z], "%s: sequences %d and %d share a cache", name, y, z);
+            LLM_REQUIRE(!meets(k_caches[y], own_bytes) && !meets(v_caches[y], own_bytes), "%s: sequences %d and %d share a cache", name, y, z);
         a.host.seq.k_cache[z] = k_caches[z];
         a.host.seq.v_cache[z] = v_caches[z];
         a.host.seq.pos[z] = positions[z];

@@ -1,5 +1,6 @@
 // Rows of a KV cache copied into the caches of other sequences, all layers and both halves in one launch.
 #include "common.hpp"
+#include "ranges.hpp"
 
 #define KF_MAX_DST LLM_MAX_BATCH
 #define KF_THREADS 256
@@ -71,11 +72,6 @@ template <bool NT_V> __global__ __launch_bounds__(KF_THREADS) void kv_fork_kerne
             for (int i = 0; i < a.n_dst; ++i) a.v_dst[i][d + q] = v;
         }
     }
-}
-
-static bool ranges_meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y + b_bytes && y < x + a_bytes;
 }
 
 extern "C" int llm_kv_fork(const uint16_t *k_src, const uint16_t *v_src, int src_max_pos, int src_row, uint16_t *const *k_dsts,

@@ -153,3 +153,26 @@ def test_logprobs_workspace_holds_smaller_calls_too(pkg):
 def test_logprobs_of_more_rows_than_can_be_counted(pkg, rows):
     """Next to the type's end the cut of a row and the loop over slices would overflow it."""
     refused(pkg, logprobs(pkg, rows=rows, vocab=1, ld=1, k=1), "at most")
+
+
+OWN = 2 * 8 * 128 * 256     # bytes of one half of an own cache of `shared` above
+PREFIX = 2 * 8 * 128 * 128  # and of the prefix cache
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(ks=(A + 3 * BIG, A + 3 * BIG + 16)), "share"), (dict(ks=(A + 3 * BIG, A + 3 * BIG + OWN - 16)), "share"),
+    (dict(vs=(A + 5 * BIG, A + 5 * BIG - OWN + 16)), "share"), (dict(vs=(A + 5 * BIG, A + 3 * BIG)), "share"),
+    (dict(vs=(A + 5 * BIG, A + 4 * BIG + 256)), "halves"), (dict(ks=(A + 3 * BIG, A + 4 * BIG), vs=(A + 3 * BIG, A + 6 * BIG)), "halves"),
+    (dict(kp=A + 3 * BIG + 16), "the prefix lies in cache 0"), (dict(vp=A + 6 * BIG + OWN - 16), "the prefix lies in cache 1"),
+    (dict(kp=A + 6 * BIG), "the prefix lies in cache 1"), (dict(vp=A + 3 * BIG), "the prefix lies in cache 0"),
+    (dict(kp=A + 4 * BIG - PREFIX + 16), "the prefix lies in cache 1"),
+    (dict(kp=A + 3 * BIG + 16, vp=A + 5 * BIG + 16, pmax=256), "the prefix lies in cache 0"),
+])
+def test_shared_attention_on_memory_in_common(pkg, over, text):
+    refused(pkg, shared(pkg, **over), text)
+
+
+def test_shared_attention_takes_caches_side_by_side(pkg):
+    """Caches that touch but do not overlap pass: these calls are refused for their positions, which are looked at cache by cache."""
+    refused(pkg, shared(pkg, ks=(A, A + OWN), vs=(A + 2 * OWN, A + 3 * OWN), kp=A + 4 * OWN, vp=A + 4 * OWN + PREFIX, pos=(100, 256)), "position 256")
+    refused(pkg, shared(pkg, ks=(A, A + OWN), vs=(A + 2 * OWN, A + 3 * OWN), kp=A, vp=A + 2 * OWN, pmax=256, pos=(100, 256)), "position 256")
