@@ -216,7 +216,7 @@ void llama3_read_batch_logits(CudaCache *cache0, int b, llm_half *logits);
  * gone.  Rows that a destination has in common with src from an earlier fork are not copied again, so an answer that branches
  * from its sibling costs its own tokens only.
  * llama3_decode_batch on caches that have rows in common reads those rows once for all sequences
- * (llm_attn_decode_rope_shared_dev) where that is faster: 512 rows or more, and 4096 or more times the batch.  The sums of the
+ * (llm_attn_decode_rope_shared_dev) where that is faster: 512 rows or more that, times the batch, are 4096 or more.  The sums of the
  * attention run in another order then.  llama3_set_shared_prefix(caches[0], mode): 0 never, 1 (default) as said, 2 with any row
  * in common.  llama3_shared_prefix_steps: batched steps with this cache as caches[0] that did. */
 void llama3_fork(CudaCache *src, CudaCache *const *dsts, int n);

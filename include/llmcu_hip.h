@@ -284,8 +284,9 @@ int llm_attn_decode_rope_batch_dev(const uint16_t *qkv_dev, int ldq, const llm_b
  * pipe with fp16 operands and fp32 accumulation, softmax statistics and sums in fp32; a softmax weight is the sum of two fp16
  * operands, within 2^-22 of itself and 2^-32 of the largest.  The order of the sums depends on the
  * lengths only: equal calls give equal bits.
- * workspace: llm_attn_shared_workspace_bytes, zeroed once with llm_fill_zero before its first use (every call leaves it
- * reusable, by calls of other shapes too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured graphs.
+ * workspace: llm_attn_shared_workspace_bytes, of any contents (a call reads nothing there that it did not write; other shapes
+ * may use it too if it is large enough for them); calls that share a workspace must not overlap, also not as nodes of two captured
+ * graphs.
  * No counterpart in the reference (it serves one sequence). */
 size_t llm_attn_shared_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int batch);
 int llm_attn_decode_rope_shared(const uint16_t *qkv_dev, int ldq, const uint16_t *k_prefix_dev, const uint16_t *v_prefix_dev,

@@ -116,8 +116,8 @@ struct Engine {
     void *b_ws_shared = nullptr;
     llm_graph_t b_shared_graph[17] = {};
     bool b_shared_ran[17] = {};
-    // log probabilities (llama3_logprobs, llama3_batch_logprobs, llama3_score): device buffers for LP_ROWS rows, a pinned
-    // mirror of the results, the logits of a scored pass
+    // log probabilities (llama3_logprobs, llama3_batch_logprobs, llama3_score): device buffers for LP_ROWS rows, the logits of a
+    // scored pass
     int32_t *lp_ids = nullptr, *lp_top_ids = nullptr;
     float *lp_out = nullptr, *lp_entropy = nullptr, *lp_top = nullptr;
     void *lp_ws = nullptr;
@@ -920,9 +920,7 @@ extern "C" void llama3_decode_batch(Llama3 *m, CudaCache *const *caches, const i
     if (prefix > 0 && (e0->shared_mode == 2 || (batch > 1 && prefix >= SHARED_FROM && batch * prefix >= SHARED_FROM_ROWS))) {
         form = SHARED_FORM;
         if (!e0->b_shared) {
-            const size_t wsb = (llm_attn_shared_workspace_bytes(Hq, c.n_kv_heads, hd, 16) + 3) / 4 * 4;
-            e0->b_ws_shared = dmalloc<char>(wsb, "llm_malloc(shared attention workspace)");
-            llama3_check(llm_fill_zero(e0->b_ws_shared, wsb, s), "zero workspace");
+            e0->b_ws_shared = dmalloc<char>(llm_attn_shared_workspace_bytes(Hq, c.n_kv_heads, hd, 16), "llm_malloc(shared attention workspace)");
             void *hp = nullptr;
             llama3_check(llm_malloc_host(&hp, sizeof(llm_shared_desc)), "llm_malloc_host(shared batch descriptor)");
             e0->b_shared_host = (llm_shared_desc *)hp;

@@ -394,3 +394,20 @@ def test_scores_of_any_magnitude(gpu, heads, prefix, scale):
                 assert np.array_equal(got[z, g * hd:(g + 1) * hd], V[:, order[-1]]), (z, g)
     say("rows with one position ahead:", seen, "of", 2 * Hq)
     assert seen >= Hq
+
+
+@pytest.mark.parametrize("fill", [0x00, 0xff, 0x7f])
+def test_a_workspace_of_any_contents(gpu, monkeypatch, fill):
+    """Zeros, NaN or large numbers in the workspace: a call reads nothing there that it did not write, in any of its forms."""
+    def filled(nbytes):
+        return gpu.capi.DevBuf.from_host(np.full(nbytes + 3 & ~3, fill, np.uint8))
+
+    for prefix, tails, heads in ((1400, [0, 17, 70, 129], (8, 2, 128)), (65, [2000, 1, 700], (8, 2, 128)), (3000, [0, 0], (4, 4, 64)),
+                                 (200, [3, 9], (8, 2, 32))):
+        c = case(34, len(tails), prefix, tails, heads, True)
+        with monkeypatch.context() as m:
+            zeroed = run(gpu, c)
+            m.setattr(gpu.ops, "_zeroed", filled)
+            assert all(np.array_equal(x, y) for x, y in zip(run(gpu, c), zeroed))
+            want = expected(c)
+            verify(run(gpu, c, dev=True, max_prefix=c["kp"].shape[1], max_tail=c["kcs"].shape[2] - 1), want)
