@@ -213,7 +213,7 @@ void llama3_read_batch_logits(CudaCache *cache0, int b, llm_half *logits);
  * llama3_fork: dsts[0..n-1] (1..16 caches of the same configuration) become copies of src: its cached rows, ids, position and
  * the logits of the last row that it processed on its own.  Each stands for itself afterwards and takes every call of this
  * interface, with the model that src was last used with (another one is refused until llama3_cache_reset); what it held before is
- * gone.  Rows that a destination has in common with src from an earlier fork are not copied again, so an answer that branches
+ * gone.  Rows that all destinations have in common with src from earlier forks are not copied again, so an answer that branches
  * from its sibling costs its own tokens only.
  * llama3_decode_batch on caches that have rows in common reads those rows once for all sequences
  * (llm_attn_decode_rope_shared_dev) where that is faster: 512 rows or more that, times the batch, are 4096 or more.  The sums of the

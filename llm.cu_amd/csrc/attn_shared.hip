@@ -12,8 +12,8 @@
 // Measured, 32 / 8 heads of 128, 16 sequences, one call (two launches): 8192 + 256 positions each 18.5 us (43 MB, 8.5 us at the
 // 5.07 TB/s of a large copy), 32768 + 1024 46.6 us (171 MB, 33.8 us); llm_attn_decode_rope_batch on caches of their own 108 us
 // at 16 x 8192.  In its steady state the first launch reads 6.3 TB/s; what is left hardly depends on the lengths: 4 to 5 us until
-// its first tiles are there, 1.5 us at its end, 5 to 6 us for the second launch and the parts in front of it (16.8 MB written and
-// read when 512 workgroups leave some for 16 sequences).
+// its first tiles are there (half of the ring holds queries and table rows first), 1.5 us at its end, 5 to 6 us for the second launch
+// and the parts in front of it (16.8 MB written and read when 512 workgroups leave some for 16 sequences).
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -80,7 +80,7 @@ template <bool DEV> __device__ __forceinline__ SharedSeq shared_seq(const Shared
 //
 // Two workgroups of four wavefronts per compute unit, each with a ring of two 32 KB stages, so that one works or begins while the
 // other waits: 45.3 / 21.0 us at 16 x (32768 + 1024) / (8192 + 256) against 47.8 / 22.8 us with one workgroup of eight
-// wavefronts and four stages.
+// wavefronts and four stages (weights in one operand, shares of two units).
 // ---------------------------------------------------------------------------------------------------------------
 #define AS_WAVES 4    // wavefronts of a workgroup
 #define AS_THREADS (64 * AS_WAVES)
@@ -115,18 +115,19 @@ template <int HD, int QT, int W> constexpr int as_lds_bytes() {
 // prefix comes from workgroup i, and workgroup i's part of tail z goes to place i + z (both only grow along the line).
 //
 // Whole tiles: in units of 8, 16 and 32 keys, whose shares are nearer to equal but end inside a tile, 16 x (32768 + 1024) took
-// 47.6, 47.4 and 46.5 us against 45.3, 16 x (8192 + 256) 23.9, 23.6 and 23.3 us against 21.0.
+// 47.6, 47.4 and 46.5 us against 45.3, 16 x (8192 + 256) 23.9, 23.6 and 23.3 us against 21.0 (weights in one operand, shares of two
+// units).
 //
 // A share's size.  A unit costs its workgroup some 1 us as long as memory is not full, a part costs every row of the merge: the
 // best size grows with the square root of the line, and with that of the KV heads, whose parts the merge reads side by side.
-// Measured with 8 heads of 128, shares of 2, 3, 4, 5, 6, 8 and 10 units: 2 x (2048 + 16) 10.9 10.8 11.6 12.4 13.2 14.9 16.6 us,
-// 2 x (4096 + 64) 12.8 11.5 11.8 12.7 13.5 15.2 16.9, 2 x (8192 + 64) 15.0 (3 units at least) 15.0 14.4 13.3 13.8 15.3 17.0,
-// 4 x (16384 + 64) 19.8 (5 at least) .. 20.1 18.0 17.9.  One KV head: 4 x (32768 + 100) 23.0 us with 2 units, 16.0 with 4, 19.7 with
-// 11.  From 16384 positions on all workgroups are wanted, at the smaller heads (half the bytes and less per unit) always: 8 heads of
-// 64, 4 x (32768 + 100) 18.1 us with 8 units, 20.0 with 11.
+// Measured with 8 heads of 128, shares of 2, 3, 4, 5, 6, 8 and 10 units: 2 x (2048 + 16) 10.7 10.8 11.5 12.4 13.3 15.2 17.0 us,
+// 2 x (4096 + 64) 12.8 11.5 11.9 12.7 13.6 15.4 17.3, 2 x (8192 + 64) 15.0 (3 units at least) 15.0 13.6 13.4 13.8 15.6 17.4,
+// 4 x (16384 + 64) 19.8 (5 at least) .. 20.3 17.6 18.2.  One KV head: 4 x (32768 + 100) 22.7 us with 2 units, 16.2 with 4, 15.3 with 5,
+// 19.5 with 11.  From 16384 positions on all workgroups are wanted, at the smaller heads (half the bytes and less per unit) always:
+// 8 heads of 64, 4 x (32768 + 100) 18.8 us with 8 units, 20.1 with 11.
 //
-// Empty units: 6, 3 where memory is full and a unit takes three times as long: with 3 and 6, 16 x (8192 + 64) 20.0 and 17.2 us,
-// 8 x (8192 + 128) 16.8 and 14.9, 16 x (32768 + 1024) 45.6 and 46.5, 8 x (2048 + 64), in shares of two, 11.6 and 12.4.
+// Empty units: 6, 3 where memory is full and a unit takes three times as long: with 3 and 6, 16 x (8192 + 64) 19.5 and 17.7 us,
+// 8 x (8192 + 128) 16.5 and 15.0, 16 x (32768 + 1024) 46.6 and 47.7, 8 x (2048 + 64), in shares of two, 11.6 and 12.5.
 #define AS_UNIT 64
 struct AsPlan {
     int wgs;            // workgroups per KV head
@@ -520,8 +521,8 @@ __global__ __launch_bounds__(AS_THREADS, AS_WAVES * AS_PER_CU / 4) void attn_sha
 }
 
 // One workgroup per query head and sequence: the parts' weights (first wavefront) and the new token's score (second one) while
-// the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.  Latency: 4.8 to 6.6 us
-// for 32 heads x 5 to 16 sequences with some 20 to 65 parts each, of which the parts' bytes would take 3.
+// the parts' rows travel, then the weighted sum.  The first head of a group appends the new key and value.  Latency: 4.5 to 6.6 us
+// for 32 or 64 heads x 5 to 16 sequences with some 20 to 65 parts each, of which the parts' bytes would take 1 to 3.
 #define AS_MERGE_THREADS 256
 // parts per thread asked for at once (80 at head size 128, more than a head of eight has)
 #define AS_MERGE_AHEAD 10
@@ -673,9 +674,9 @@ __global__ __launch_bounds__(64 * AS_DIRECT_WAVES) void attn_shared_direct_kerne
 }
 
 // Tiles (128 keys at head size 128, 256 at the others) up to which that is faster than two launches, one more at the smaller
-// head sizes.  Measured on 1, 4 and 16 sequences, direct against parts: head size 128, four tiles 10.5 / 10.6 / 10.8 against 10.8 /
-// 10.8 / 12.7 us, five 11.9 / 12.0 / 12.1 against 10.8 / 10.8 / 12.7; head size 64, five 10.5 / 10.6 / 10.6 against 10.8 / 10.8 / 10.9,
-// six 11.8 / 11.9 / 11.9 against 10.8 / 10.8 / 10.9; head size 32, five 8.4 / 8.6 / 8.7 against 10.8.
+// head sizes.  Measured on 1, 4 and 16 sequences, direct against parts: head size 128, four tiles 10.7 / 10.8 / 10.9 against 10.8 /
+// 10.9 / 12.9 us, five 12.1 / 12.1 / 12.3 against 10.9 / 10.9 / 13.1; head size 64, five 10.7 / 10.8 / 10.8 against 10.9 / 10.9 / 11.1,
+// six 12.0 / 12.0 / 12.1 against 10.9 / 10.9 / 11.0; head size 32, five 8.6 / 8.8 / 8.8 against 10.9 / 10.9 / 11.0.
 #define AS_DIRECT_TILES 4
 // Workgroups per KV head: two on each of the 256 compute units.
 static int as_wgs(int n_kv_heads) { return n_kv_heads < 256 * AS_PER_CU ? 256 * AS_PER_CU / n_kv_heads : 1; }

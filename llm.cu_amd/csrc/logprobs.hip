@@ -8,9 +8,9 @@
 // a row that finishes last joins the chunks.
 //
 // What bounds it: many rows, the logits' bytes (read once): 2048 rows of 128256, the best alternative and one given token 96 us,
-// 5.5 TB/s (a large copy reads and writes 5.07); the 20 best 120 us, what listing candidates and cutting the lists adds.  Few
-// rows, latency: 16 rows, 5 best 8.6 us, one row, 20 best 10.1 us, of which an empty launch through the same call is 7; on the
-// chip alone one row takes 5.0 us without alternatives, some 5 more with 20: the two levels of lists.
+// 5.5 TB/s (a large copy reads and writes 5.07); the 20 best 125 us, what listing candidates and cutting the lists adds to the six
+// operations a logit.  Few rows, the kernel's latency: 16 rows, 5 best, 8.5 us, one row, 20 best, 10.2 us a call (10.6 on the chip), of
+// which 4.7 are the row without alternatives and 6 the two levels of lists; a chunk of 2048 alone takes 2.2 and, with 20, 5.2.
 //
 // Sums: exponentials are base 2, 2^((x - m) c) with c = log2(e) / temperature for the largest logit m so far.  The difference comes
 // first: it is exact or rounded once, so the largest logit has weight 1 at any temperature (a fused x c - m c is off by the rounding
@@ -37,8 +37,8 @@
 #define LP_WORKGROUPS 512      // aimed at
 #define LP_LINE 32             // ints from one row's counter to the next: device-scope additions to one line wait for one another
 #define LP_LIST 768            // words of a wavefront's list: a row of 16-byte loads (512 logits) behind what it holds
-// Lanes above the bound up to which it stays, rather than being found anew.  With 0, 3, 8 and 16: 256 rows of 128256, 5 best, 26.5
-// 25.5 28.2 30.3 us, 2048 rows 102.1 101.8 110.4 120.1; 20 best, 700 rows, 57.7 55.6 56.3 61.4.
+// Lanes above the bound up to which it stays, rather than being found anew.  With 0, 3, 8 and 16: 256 rows of 128256, 5 best, 27.1
+// 26.1 28.7 30.8 us, 2048 rows 106.5 106.9 115.6 123.9; 20 best, 700 rows, 59.8 57.8 58.9 63.6.
 #define LP_FEW 3
 #define LP_JOIN (LP_MAX_CHUNKS * LP_MAX_TOP / LP_THREADS) // listed logits per thread when chunks are joined
 #define LP_LOWEST 0x0400u      // order key of -65504, the lowest logit that has a probability
@@ -414,10 +414,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
 
 // How a row is cut.  Few rows: finely, so that their logits come from many compute units at once, but into LP_MAX_CHUNKS pieces
 // at most; many rows: coarsely, so that less is joined.  Aimed at LP_WORKGROUPS; with 256, 512 and 1024, rows of 128256: 64 rows,
-// 20 best, 21.2 18.1 17.1 us, 256 rows, 5 best, 28.5 24.6 23.4, but 700 rows, 20 best, 54 54 69.
+// 20 best, 21.0 17.8 15.9 us, 256 rows, 5 best, 30.1 26.1 24.8, but 700 rows, 20 best, 58 58 69.
 // Short chunks in short segments, so that all wavefronts have one, long chunks in long ones with more loads in flight: with 1, 2
-// and 4 loads per lane 16 rows (chunks of 4096) 9.7 9.0 9.3 us, one row (2048) 8.4 and, with 4, 9.3, 2048 whole rows 110 with one
-// and 101 with 4 (5 best).
+// and 4 loads per lane 16 rows (chunks of 4096), 5 best, 9.5 8.5 8.9 us, one row (2048), 20 best, 10.2 and, with 4, 11.8, 2048 whole
+// rows, 5 best, 115 with one and 107 with 4.
 struct LpCut {
     int nl, chunk_len, chunks;
 };

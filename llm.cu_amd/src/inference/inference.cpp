@@ -134,8 +134,8 @@ constexpr int ROPE_IN_ATTENTION_FROM = 4096;
 
 // Batched steps of forks read the shared prefix once for all from this many shared positions on, and where batch times
 // positions makes up for the second launch.  Measured, attention of a layer (8B heads), every cache for itself against shared:
-// 2 sequences, 1024 positions 10.3 against 11.8 us, 2048 12.8 against 12.1; 4 sequences, 512 10.7 against 11.9, 1024 12.8 against
-// 11.9; 8 sequences, 512 14.5 against 12.0; 16 sequences, 256 11.9 against 13.8, 512 21.8 against 14.0, 8192 108 against 18.2.
+// 2 sequences, 1024 positions 10.3 against 11.6 us, 2048 12.8 against 12.0; 4 sequences, 512 10.7 against 11.6, 1024 12.7 against
+// 11.8; 8 sequences, 512 14.5 against 11.9; 16 sequences, 256 12.0 against 13.9, 512 21.7 against 14.4, 8192 108 against 19.5.
 constexpr int SHARED_FROM = 512, SHARED_FROM_ROWS = 4096;
 constexpr size_t MAX_MARKS = 8;
 constexpr int LP_ROWS = 512; // rows of logits that llama3_score holds at a time
