@@ -285,13 +285,17 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs a) {
         if (__builtin_amdgcn_ballot_w64((float)top > st.m)) st = lp_rebase(st, fmaxf(st.m, wave_max((float)top)), c);
         const float base = lp_base(st.m);
 #pragma unroll
-        for (int u = 0; u < NL; ++u)
+        for (int u = 0; u < NL; ++u) {
+            float p[8], t = 0.f; // eight at a time: a lane's sums take an eighth of the roundings one after the other
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float d = fmaf((float)v[u][e], one, -base), p = __builtin_amdgcn_exp2f(d * c);
-                st.s += p;
-                st.t = fmaf(fmaxf(d, -FLT_MAX), p, st.t); // -inf times zero is zero here; a NaN is in p already
+                const float d = fmaf((float)v[u][e], one, -base);
+                p[e] = __builtin_amdgcn_exp2f(d * c);
+                t = fmaf(fmaxf(d, -FLT_MAX), p[e], t); // -inf times zero is zero here; a NaN is in p already
             }
+            st.s += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            st.t += t;
+        }
         lane_best = top > lane_best ? top : lane_best;
         const int lanes = k > 0 ? __popcll(__builtin_amdgcn_ballot_w64(top >= from)) : 0;
         if (lanes) {
