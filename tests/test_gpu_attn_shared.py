@@ -411,3 +411,17 @@ def test_a_workspace_of_any_contents(gpu, monkeypatch, fill):
             assert all(np.array_equal(x, y) for x, y in zip(run(gpu, c), zeroed))
             want = expected(c)
             verify(run(gpu, c, dev=True, max_prefix=c["kp"].shape[1], max_tail=c["kcs"].shape[2] - 1), want)
+
+
+@pytest.mark.parametrize("prefix,row0", [(200, 1), (200, 7), (200, 64), (200, 199), (1400, 8), (1400, 199), (1400, 1300)])
+def test_own_caches_that_begin_inside_the_prefix(gpu, prefix, row0):
+    """Row 0 of the own caches is a position of the prefix: their rows in front of the prefix's end are not read."""
+    lead = prefix - row0
+    c = case(35, 3, prefix, [0, 17, 130], (8, 2, 128), True, own_slack=lead)
+    kcs, vcs = np.full_like(c["kcs"], NAN), np.full_like(c["vcs"], NAN)
+    kcs[:, :, lead:lead + 130], vcs[:, :, :, lead:lead + 130] = c["kcs"][:, :, :130], c["vcs"][:, :, :, :130]
+    c.update(kcs=kcs, vcs=vcs, row0=row0)
+    say("prefix", prefix, "row 0 at", row0)
+    want = closely(c)
+    verify(run(gpu, c), want)
+    verify(run(gpu, c, dev=True, max_prefix=c["kp"].shape[1], max_tail=kcs.shape[2] - 1), want)
